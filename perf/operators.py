@@ -267,7 +267,7 @@ def _own(case, s):
 
     if case["kind"] == "bias":
         return {"bias": ops.relative_bias(s["table"], s["plan"], case["Sq"], case["Sk"], q_start=case["q_start"]),
-                "dtable": ops.relative_bias_backward(s["dbias"], s["plan"], q_start=case["q_start"])}
+                "dtable": ops.relative_bias_backward(s["dbias"], s["plan"], case["buckets"], q_start=case["q_start"])}
     how = dict(kv_heads=case["kv_heads"], causal=case["causal"], q_start=case["q_start"], key_mask=s["mask"], key_count=s["count"],
                scale=_scale(case), rel_bias=(s["table"], s["plan"]) if case["bias"] else None)
     if case["kind"] == "attend":
