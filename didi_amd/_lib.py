@@ -20,6 +20,7 @@ i64p = C.POINTER(C.c_int64)
 OK = 0
 PREC_BF16, PREC_FP16, PREC_BF16X3, PREC_FP16X2, PREC_FP16X3 = 1, 2, 3, 4, 5
 FMT_BF16, FMT_FP16 = 0, 1
+DT_BF16, DT_FP16, DT_FP32 = 0, 1, 2
 ACT_NONE, ACT_GELU, ACT_TANH, ACT_RELU, ACT_GELU_NEW = 0, 1, 2, 3, 4
 STEP_NONE, STEP_INIT, STEP_DDPM, STEP_EULER = 0, 1, 2, 3
 ERR_FAULT = -5
@@ -73,6 +74,23 @@ class AttnTrainArgs(C.Structure):
         ("ldq", C.c_int), ("ldk", C.c_int), ("ldv", C.c_int), ("ldo", C.c_int), ("causal", C.c_int),
         ("scale", C.c_float), ("drop_p", C.c_float), ("seed", C.c_uint64), ("offset", C.c_uint64),
         ("O", C.c_void_p), ("dQ", C.c_void_p), ("dK", C.c_void_p), ("dV", C.c_void_p), ("pos_bias", C.c_void_p),
+    ]
+
+
+class LongAttnArgs(C.Structure):
+    _fields_ = [
+        ("B", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("Sq", C.c_int), ("Sk", C.c_int), ("D", C.c_int),
+        ("dtype", C.c_int), ("causal", C.c_int), ("q_start", C.c_int), ("scale", C.c_float),
+        ("key_mask", C.c_void_p), ("key_count", C.c_void_p),
+        ("Q", C.c_void_p), ("K", C.c_void_p), ("V", C.c_void_p), ("Q_lo", C.c_void_p), ("K_lo", C.c_void_p), ("V_lo", C.c_void_p),
+        ("q_batch", C.c_int64), ("k_batch", C.c_int64), ("v_batch", C.c_int64), ("ldq", C.c_int), ("ldk", C.c_int), ("ldv", C.c_int),
+        ("O", C.c_void_p), ("O_lo", C.c_void_p), ("o_batch", C.c_int64), ("ldo", C.c_int), ("lse", C.c_void_p),
+        ("table", C.c_void_p), ("buckets", C.c_void_p), ("num_buckets", C.c_int), ("max_distance", C.c_int),
+        ("drop_p", C.c_float), ("seed", C.c_uint64), ("offset", C.c_uint64),
+        ("dO", C.c_void_p), ("do_batch", C.c_int64), ("lddo", C.c_int),
+        ("dQ", C.c_void_p), ("dK", C.c_void_p), ("dV", C.c_void_p), ("dq_batch", C.c_int64), ("dk_batch", C.c_int64), ("dv_batch", C.c_int64),
+        ("lddq", C.c_int), ("lddk", C.c_int), ("lddv", C.c_int),
+        ("dtable", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -219,6 +237,13 @@ SYMBOLS = [
     ("didi_seq_sum", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     ("didi_train_target_backward", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_float, C.c_float, C.c_void_p,
                                              C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
+    ("didi_long_attention_workspace_bytes", C.c_size_t, [C.POINTER(LongAttnArgs), C.c_int]),
+    ("didi_long_attention_forward", C.c_int, [C.POINTER(LongAttnArgs), C.c_void_p]),
+    ("didi_long_attention_backward", C.c_int, [C.POINTER(LongAttnArgs), C.c_void_p]),
+    ("didi_relative_bias", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
+    ("didi_relative_bias_backward_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    ("didi_relative_bias_backward", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
+                                              C.c_void_p, C.c_void_p]),
     ("didi_event_create", C.c_int, [C.POINTER(C.c_void_p)]),
     ("didi_event_elapsed_ms", C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_float)]),
     ("didi_event_destroy", C.c_int, [C.c_void_p]),

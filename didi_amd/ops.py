@@ -628,3 +628,170 @@ def train_target_backward(x0hat, emb, x0, mask, w_emb, w_x0, w_T, c_b, dxt, extr
                                               _lib.ptr(None if extra is None else _f32c(extra)), B, S, H, out.data_ptr(),
                                               _lib.current_stream()), "train_target_backward")
     return out
+
+
+# ------------------------------------------------------------------ attention of any lengths, learned relative position bias
+_DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_FP16, torch.float32: _lib.DT_FP32}
+
+
+def _on(dev):
+    """Context in which ``dev`` is the current device (kernels are launched on its current stream)."""
+    import contextlib
+
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
+    """The bucket of every distance key - query from -max_distance to max_distance -> int32 [2 max_distance + 1]; farther distances
+    share the end's.  T5's rule (HF:models/t5/modeling_t5.py:217-266) in whole numbers: half of a side's buckets hold one distance each, the
+    k-th of the n others starts at the first distance with d ** n * exact ** k >= exact ** n * max_distance ** k.  ``bidirectional`` False: only
+    what lies before the query is told apart.  A model computes it once and keeps it beside its table [num_buckets, heads]."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    exact = side // 2
+    if exact < 1 or (bidirectional and num_buckets % 2) or max_distance <= exact:
+        raise ValueError(f"num_buckets={num_buckets} with max_distance={max_distance}: at least {4 if bidirectional else 2} buckets (an even number on "
+                         "two sides), and a max_distance beyond the buckets of one distance each")
+    n, k, bucket = side - exact, 0, []
+    for d in range(max_distance + 1):
+        while k + 1 < n and d >= exact and d ** n * exact ** (k + 1) >= exact ** n * max_distance ** (k + 1):
+            k += 1
+        bucket.append(d if d < exact else exact + k)
+    after = [side + b for b in bucket[1:]] if bidirectional else [0] * max_distance
+    return torch.tensor(bucket[:0:-1] + bucket[:1] + after, dtype=torch.int32).to(device)
+
+
+def _check_buckets(buckets, device):
+    if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0 or not buckets.is_contiguous() or buckets.device != device:
+        raise ValueError(f"buckets must be what relative_buckets returns (int32, an odd number of distances, on {device})")
+    return buckets.numel() // 2
+
+
+def relative_bias(table, buckets, Sq, Sk, q_start=0):
+    """The dense bias [heads, Sq, Sk] = table[buckets[j - i - q_start]] of a learned table [num_buckets, heads] (bf16, fp16 or fp32)."""
+    if table.dtype not in _DT or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("table must be a contiguous bf16, fp16 or fp32 [num_buckets, heads]")
+    maxd = _check_buckets(buckets, table.device)
+    nb, heads = table.shape
+    with _on(table.device):
+        out = torch.empty((heads, Sq, Sk), dtype=table.dtype, device=table.device)
+        _lib.check(lib.didi_relative_bias(table.data_ptr(), buckets.data_ptr(), _DT[table.dtype], heads, nb, maxd, Sq, Sk, q_start, out.data_ptr(),
+                                          _lib.current_stream()), "relative_bias")
+    return out
+
+
+def relative_bias_backward(dbias, buckets, num_buckets, q_start=0):
+    """Gradient of the table [num_buckets, heads] from that of the dense bias: dbias [heads, Sq, Sk], or [B, heads, Sq, Sk] of the B dialogs
+    that shared it.  Deterministic."""
+    if dbias.dtype not in _DT or dbias.dim() not in (3, 4) or not dbias.is_contiguous():
+        raise ValueError("dbias must be a contiguous bf16, fp16 or fp32 [heads, Sq, Sk] or [B, heads, Sq, Sk]")
+    maxd = _check_buckets(buckets, dbias.device)
+    B, heads, Sq, Sk = (1, *dbias.shape) if dbias.dim() == 3 else dbias.shape
+    with _on(dbias.device):
+        dtable = torch.empty((num_buckets, heads), dtype=dbias.dtype, device=dbias.device)
+        ws = torch.empty(lib.didi_relative_bias_backward_bytes(B, heads, maxd, Sq), dtype=torch.uint8, device=dbias.device)
+        _lib.check(lib.didi_relative_bias_backward(dbias.data_ptr(), buckets.data_ptr(), _DT[dbias.dtype], B, heads, num_buckets, maxd, Sq, Sk, q_start,
+                                                   dtable.data_ptr(), ws.data_ptr(), _lib.current_stream()), "relative_bias_backward")
+    return dtable
+
+
+def _long_rows(name, t, B, S, W, dtype, device):
+    """Checks a [B, S, W] operand -> (address, elements between dialogs, between rows)."""
+    if t.shape != (B, S, W) or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} [{B}, {S}, {W}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if W > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: neighbouring columns must be neighbours in memory (strides {t.stride()})")
+    return t.data_ptr(), (t.stride(0) if B > 1 else 0), (t.stride(1) if S > 1 else W)
+
+
+def _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset):
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in _DT or not q.is_cuda:
+        raise ValueError("q, k, v must be bf16, fp16 or fp32 [B, S, heads D] tensors on the GPU")
+    B, Sq, HD = q.shape
+    Sk = k.shape[1]
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or HD % heads:
+        raise ValueError(f"heads={heads} must divide the width {HD} and be a multiple of kv_heads={kv_heads}")
+    if scale is not None and not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale={scale} must be positive and finite")
+    D, dt, dev = HD // heads, q.dtype, q.device
+    a = _lib.LongAttnArgs(B, heads, kv_heads, Sq, Sk, D, _DT[dt], int(causal), q_start, 0.0 if scale is None else scale)
+    a.Q, a.q_batch, a.ldq = _long_rows("q", q, B, Sq, HD, dt, dev)
+    a.K, a.k_batch, a.ldk = _long_rows("k", k, B, Sk, kv_heads * D, dt, dev)
+    a.V, a.v_batch, a.ldv = _long_rows("v", v, B, Sk, kv_heads * D, dt, dev)
+    for name, m, shape in (("key_mask", key_mask, (B, Sk)), ("key_count", key_count, (B,))):
+        if m is not None:
+            if m.dtype != torch.int32 or m.shape != shape or not m.is_contiguous() or m.device != dev:
+                raise ValueError(f"{name} must be a contiguous int32 {list(shape)} on {dev}")
+            setattr(a, name, m.data_ptr())
+    if rel_bias is not None:
+        table, buckets = rel_bias
+        if table.dtype != dt or table.dim() != 2 or table.shape[1] != heads or not table.is_contiguous() or table.device != dev:
+            raise ValueError(f"rel_bias = (table, buckets): the table must be a contiguous {dt} [num_buckets, {heads}] on {dev}")
+        a.max_distance = _check_buckets(buckets, dev)
+        a.table, a.buckets, a.num_buckets = table.data_ptr(), buckets.data_ptr(), table.shape[0]
+    if drop_p:
+        a.drop_p, a.seed, a.offset = drop_p, seed, offset
+    return a
+
+
+def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_mask=None, key_count=None, scale=None, rel_bias=None, drop_p=0.0,
+                    seed=0, offset=0, need_grad=False, out=None):
+    """Attention of q [B, Sq, heads D] over k, v [B, Sk, kv_heads D] of any other length (self-attention: the same sequence) -> o like q.
+
+    bf16, fp16 or fp32, all operands alike; views with strides between rows and dialogs are fine (16-byte aligned).  Head dims up to 128,
+    multiples of 8 (fp32: 4).  ``kv_heads``: each key head serves heads / kv_heads query heads.  A key is visible where
+    ``key_mask`` int32 [B, Sk] is not 0, before ``key_count`` int32 [B], and (``causal``) up to position q_start + i; a row that sees none
+    gives zeros, and what lies at invisible keys is never used.  ``scale``: default 1/sqrt(D).  ``rel_bias`` = (table [num_buckets, heads],
+    relative_buckets(...)): a learned bias by the distance from query q_start + i to the key, added to the scaled scores.  ``drop_p``,
+    ``seed``, ``offset``: dropout of the probabilities, ``attention_train``'s mask.
+    ``need_grad``: -> (o, saved) for ``cross_attention_backward``.  ``out``: written in place (its strides as q's)."""
+    a = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
+    dev, B, Sq = q.device, a.B, a.Sq
+    with _on(dev):
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+        a.O, a.o_batch, a.ldo = _long_rows("out", o, B, Sq, q.shape[2], q.dtype, dev)
+        saved = None
+        if need_grad:
+            # the output's remainder plane: the bias gradient's sums cancel and want D = do . o beyond o's own 8 or 11 bits
+            o_lo = torch.empty_strided(o.shape, o.stride(), dtype=q.dtype, device=dev) if rel_bias is not None and q.dtype != torch.float32 else None
+            saved = (torch.empty((B, heads, Sq), dtype=torch.float32, device=dev), o_lo)
+            a.lse, a.O_lo = saved[0].data_ptr(), _lib.ptr(o_lo)
+        nbytes = lib.didi_long_attention_workspace_bytes(a, 0)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+        _lib.check(lib.didi_long_attention_forward(a, _lib.current_stream()), "cross_attention")
+    return (o, saved) if need_grad else o
+
+
+def cross_attention_backward(q, k, v, o, saved, dO, heads, kv_heads=None, causal=False, q_start=0, key_mask=None, key_count=None, scale=None,
+                             rel_bias=None, drop_p=0.0, seed=0, offset=0, out=None):
+    """Backward of ``cross_attention(..., need_grad=True)`` with the same arguments -> (dq, dk, dv), and dtable where a bias was given.
+    ``out`` = (dq, dk, dv): views to write into (e.g. the thirds of a fused projection's gradient); default fresh contiguous tensors.
+    Deterministic."""
+    a = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
+    dev, dt, B, Sq, Sk = q.device, q.dtype, a.B, a.Sq, a.Sk
+    lse, o_lo = saved
+    if lse.shape != (B, heads, Sq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError("saved must be what cross_attention returned for these operands")
+    with _on(dev):
+        a.O, a.o_batch, a.ldo = _long_rows("o", o, B, Sq, q.shape[2], dt, dev)
+        if o_lo is not None:
+            if o_lo.shape != o.shape or o_lo.stride() != o.stride():
+                raise ValueError("o must be the tensor (or a copy of its layout) that cross_attention returned")
+            a.O_lo = o_lo.data_ptr()
+        a.lse = lse.data_ptr()
+        a.dO, a.do_batch, a.lddo = _long_rows("dO", dO, B, Sq, q.shape[2], dt, dev)
+        grads = tuple(torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k, v)) if out is None else tuple(out)
+        a.dQ, a.dq_batch, a.lddq = _long_rows("dq", grads[0], B, Sq, q.shape[2], dt, dev)
+        a.dK, a.dk_batch, a.lddk = _long_rows("dk", grads[1], B, Sk, k.shape[2], dt, dev)
+        a.dV, a.dv_batch, a.lddv = _long_rows("dv", grads[2], B, Sk, k.shape[2], dt, dev)
+        if rel_bias is not None:
+            grads += (torch.empty_like(rel_bias[0]),)
+            a.dtable = grads[3].data_ptr()
+        nbytes = lib.didi_long_attention_workspace_bytes(a, 1)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+        _lib.check(lib.didi_long_attention_backward(a, _lib.current_stream()), "cross_attention_backward")
+    return grads

@@ -689,6 +689,64 @@ int didi_seq_sum(const float* x, int B, int S, int H, float* out, void* stream);
 int didi_train_target_backward(const float* x0hat, const float* emb, const float* x0, const int64_t* mask, float w_emb, float w_x0, float w_T,
                                const float* c_b, const float* dxt, const float* extra, int B, int S, int H, float* out, void* stream);
 
+/* ---- attention of any lengths (no counterpart with lengths this long in didi_attention / didi_attention_train_*) ------------------
+ * Queries [B, Sq, heads D] over keys / values [B, Sk, kv_heads D] of another length: BertCrossAttention / BertSelfAttention beyond 96
+ * positions (HF:models/bert/modeling_bert.py:111-279), T5Attention with its learned relative bias (HF:models/t5/modeling_t5.py:217-279).
+ *   visible(b, i, j) = j < key_count[b] and key_mask[b, j] != 0 and (not causal or j <= q_start + i)
+ *   o_i = sum_j p_ij v_j,  p = dropout(softmax_j(scale q_i . k_j + table[buckets[clamp(j - q_start - i)]][head])) over the visible j
+ * A row that sees no key gives o = 0, lse = -inf and no gradients (didi_attention's rows without a visible key average all values
+ * instead); keys and values that are not visible to a dialog are never multiplied, whatever they hold.  Statistics and sums are fp32.
+ * dtype BF16 / FP16: one product per pair, probabilities and score gradients rounded to that type; FP32: fp32 products throughout.
+ * Q_lo, K_lo, V_lo (forward, BF16 / FP16, all three or none): split planes, joined and multiplied in fp32.
+ * O_lo (BF16 / FP16, optional): the output's remainder plane; the backward adds it to O where it is given, which the gradient of the bias
+ * table wants (its sums cancel).  Strides in elements: ld* between rows, *_batch between dialogs (inputs may repeat a dialog with 0).
+ * 16-byte aligned bases and strides (planes: 8).  D % 8 == 0 (FP32 and planes: % 4), D <= 128; max_distance <= 512, num_buckets <= 1024.
+ * Any of B, Sq, Sk may be 0.  Neither call has atomics whose order could change a result.
+ * workspace: didi_long_attention_workspace_bytes(args, backward) bytes, 16-byte aligned, NULL where that is 0.  Its size depends on the shape
+ * fields, table, dtable and dtype alone. */
+enum { DIDI_DT_BF16 = 0, DIDI_DT_FP16 = 1, DIDI_DT_FP32 = 2 };
+typedef struct didi_long_attn_args {
+    int B, heads, kv_heads, Sq, Sk, D;
+    int dtype;
+    int causal, q_start;       /* query i stands at position q_start + i (causal limit and distances) */
+    float scale;               /* 0 = 1/sqrt(D) */
+    const int32_t* key_mask;   /* [B, Sk] or NULL */
+    const int32_t* key_count;  /* [B] or NULL: keys from key_count[b] on are not visible */
+    const void *Q, *K, *V;
+    const void *Q_lo, *K_lo, *V_lo;
+    int64_t q_batch, k_batch, v_batch;
+    int ldq, ldk, ldv;
+    void *O, *O_lo;            /* backward: read */
+    int64_t o_batch;
+    int ldo;
+    float* lse;                /* [B, heads, Sq] log sum exp of the visible scores: written by the forward (NULL: not), read by the backward */
+    const void* table;         /* [num_buckets, heads] in dtype, or NULL: no bias */
+    const int32_t* buckets;    /* [2 max_distance + 1]: bucket of distance d = key - query position at [d + max_distance], farther ones as the
+                                  ends; a bucket outside the table gives NaN */
+    int num_buckets, max_distance;
+    float drop_p;              /* didi_attention_train_forward's mask stream */
+    uint64_t seed, offset;
+    const void* dO;
+    int64_t do_batch;
+    int lddo;
+    void *dQ, *dK, *dV;
+    int64_t dq_batch, dk_batch, dv_batch;
+    int lddq, lddk, lddv;
+    void* dtable;              /* [num_buckets, heads] in dtype, or NULL */
+    void* workspace;
+    size_t workspace_bytes;
+} didi_long_attn_args;
+size_t didi_long_attention_workspace_bytes(const didi_long_attn_args* a, int backward);
+int didi_long_attention_forward(const didi_long_attn_args* a, void* stream);
+int didi_long_attention_backward(const didi_long_attn_args* a, void* stream);
+/* The learned relative position bias on its own (T5Attention.compute_bias): out [heads, Sq, Sk] = table[buckets[clamp(j - q_start - i)]][h],
+ * and the table's gradient from a dense one [B, heads, Sq, Sk] (summed over the B dialogs the bias was shared by).  dtype: all operands. */
+int didi_relative_bias(const void* table, const int32_t* buckets, int dtype, int heads, int num_buckets, int max_distance, int Sq, int Sk, int q_start,
+                       void* out, void* stream);
+size_t didi_relative_bias_backward_bytes(int B, int heads, int max_distance, int Sq);
+int didi_relative_bias_backward(const void* dbias, const int32_t* buckets, int dtype, int B, int heads, int num_buckets, int max_distance, int Sq, int Sk,
+                                int q_start, void* dtable, void* workspace, void* stream);
+
 /* hipEvent wrappers for the prof_events_host hook (bench.py): events must live in the HIP runtime
  * instance this library is bound to.  Host-side helpers, no reference counterpart.  Elapsed time
  * may only be read after the caller has synchronised the stream. */
