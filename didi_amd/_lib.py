@@ -306,6 +306,12 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def raw_stream(device_index):
+    """The current stream of a device as an integer, without building a stream object (a tenth of current_stream's time: it counts where a
+    call's kernels take a few microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def current_stream():
     import torch
 

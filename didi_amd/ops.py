@@ -5,6 +5,7 @@ below passes raw device pointers to libdidi_hip and returns torch tensors that a
 Nothing falls back to eager torch arithmetic.
 """
 import ctypes as C
+import struct
 
 import torch
 
@@ -634,11 +635,13 @@ def train_target_backward(x0hat, emb, x0, mask, w_emb, w_x0, w_T, c_b, dxt, extr
 _DT = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_FP16, torch.float32: _lib.DT_FP32}
 
 
-def _on(dev):
-    """Context in which ``dev`` is the current device (kernels are launched on its current stream)."""
-    import contextlib
-
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev, fn, *args):
+    """fn(*args, current stream of dev) with dev the current device."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        return fn(*args, _lib.raw_stream(index))
+    with torch.cuda.device(dev):
+        return fn(*args, _lib.raw_stream(index))
 
 
 def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
@@ -668,70 +671,102 @@ def _check_buckets(buckets, device):
 
 def relative_bias(table, buckets, Sq, Sk, q_start=0):
     """The dense bias [heads, Sq, Sk] = table[buckets[j - i - q_start]] of a learned table [num_buckets, heads] (bf16, fp16 or fp32)."""
-    if table.dtype not in _DT or table.dim() != 2 or not table.is_contiguous():
+    dt = _DT.get(table.dtype)
+    if dt is None or table.dim() != 2 or not table.is_contiguous():
         raise ValueError("table must be a contiguous bf16, fp16 or fp32 [num_buckets, heads]")
-    maxd = _check_buckets(buckets, table.device)
+    dev = table.device
+    maxd = _check_buckets(buckets, dev)
     nb, heads = table.shape
-    with _on(table.device):
-        out = torch.empty((heads, Sq, Sk), dtype=table.dtype, device=table.device)
-        _lib.check(lib.didi_relative_bias(table.data_ptr(), buckets.data_ptr(), _DT[table.dtype], heads, nb, maxd, Sq, Sk, q_start, out.data_ptr(),
-                                          _lib.current_stream()), "relative_bias")
+    if not table.is_cuda:
+        raise ValueError("table must be on the GPU")
+    out = torch.empty((heads, Sq, Sk), dtype=table.dtype, device=dev)
+    _lib.check(_launch(dev, lib.didi_relative_bias, table.data_ptr(), buckets.data_ptr(), dt, heads, nb, maxd, Sq, Sk, q_start, out.data_ptr()), "relative_bias")
     return out
 
 
 def relative_bias_backward(dbias, buckets, num_buckets, q_start=0):
     """Gradient of the table [num_buckets, heads] from that of the dense bias: dbias [heads, Sq, Sk], or [B, heads, Sq, Sk] of the B dialogs
     that shared it.  Deterministic."""
-    if dbias.dtype not in _DT or dbias.dim() not in (3, 4) or not dbias.is_contiguous():
+    dt = _DT.get(dbias.dtype)
+    if dt is None or dbias.dim() not in (3, 4) or not dbias.is_contiguous():
         raise ValueError("dbias must be a contiguous bf16, fp16 or fp32 [heads, Sq, Sk] or [B, heads, Sq, Sk]")
-    maxd = _check_buckets(buckets, dbias.device)
+    dev = dbias.device
+    maxd = _check_buckets(buckets, dev)
+    if not dbias.is_cuda:
+        raise ValueError("dbias must be on the GPU")
     B, heads, Sq, Sk = (1, *dbias.shape) if dbias.dim() == 3 else dbias.shape
-    with _on(dbias.device):
-        dtable = torch.empty((num_buckets, heads), dtype=dbias.dtype, device=dbias.device)
-        ws = torch.empty(lib.didi_relative_bias_backward_bytes(B, heads, maxd, Sq), dtype=torch.uint8, device=dbias.device)
-        _lib.check(lib.didi_relative_bias_backward(dbias.data_ptr(), buckets.data_ptr(), _DT[dbias.dtype], B, heads, num_buckets, maxd, Sq, Sk, q_start,
-                                                   dtable.data_ptr(), ws.data_ptr(), _lib.current_stream()), "relative_bias_backward")
+    dtable = torch.empty((num_buckets, heads), dtype=dbias.dtype, device=dev)
+    ws = torch.empty(lib.didi_relative_bias_backward_bytes(B, heads, maxd, Sq), dtype=torch.uint8, device=dev)
+    _lib.check(_launch(dev, lib.didi_relative_bias_backward, dbias.data_ptr(), buckets.data_ptr(), dt, B, heads, num_buckets, maxd, Sq, Sk, q_start,
+                       dtable.data_ptr(), ws.data_ptr()), "relative_bias_backward")
     return dtable
 
 
-def _long_rows(name, t, B, S, W, dtype, device):
+def _rows(name, t, shape, dtype, device):
     """Checks a [B, S, W] operand -> (address, elements between dialogs, between rows)."""
-    if t.shape != (B, S, W) or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {dtype} [{B}, {S}, {W}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    if W > 1 and t.stride(2) != 1:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    batch, row, col = t.stride()
+    B, S, W = shape
+    if col != 1 and W > 1:
         raise ValueError(f"{name}: neighbouring columns must be neighbours in memory (strides {t.stride()})")
-    return t.data_ptr(), (t.stride(0) if B > 1 else 0), (t.stride(1) if S > 1 else W)
+    return t.data_ptr(), batch if B > 1 else 0, row if S > 1 else W
+
+
+_PACK = struct.Struct("@9if2P3P3P3q3i2PqiP2P2if2QPqi3P3q3iPPN").pack  # didi_long_attn_args
+_NO_GRADS = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
 def _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset):
-    if q.dim() != 3 or k.dim() != 3 or q.dtype not in _DT or not q.is_cuda:
+    """Checks what forward and backward share -> (B, Sq, Sk, their fields of didi_long_attn_args up to the output, those after it)."""
+    dt, dev = q.dtype, q.device
+    code = _DT.get(dt)
+    if code is None or q.dim() != 3 or k.dim() != 3 or not q.is_cuda:
         raise ValueError("q, k, v must be bf16, fp16 or fp32 [B, S, heads D] tensors on the GPU")
-    B, Sq, HD = q.shape
+    B, Sq, HD = shape = q.shape
     Sk = k.shape[1]
-    kv_heads = heads if kv_heads is None else kv_heads
+    if kv_heads is None:
+        kv_heads = heads
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads or HD % heads:
         raise ValueError(f"heads={heads} must divide the width {HD} and be a multiple of kv_heads={kv_heads}")
-    if scale is not None and not 0.0 < scale < float("inf"):
+    if scale is None:
+        scale = 0.0
+    elif not 0.0 < scale < float("inf"):
         raise ValueError(f"scale={scale} must be positive and finite")
-    D, dt, dev = HD // heads, q.dtype, q.device
-    a = _lib.LongAttnArgs(B, heads, kv_heads, Sq, Sk, D, _DT[dt], int(causal), q_start, 0.0 if scale is None else scale)
-    a.Q, a.q_batch, a.ldq = _long_rows("q", q, B, Sq, HD, dt, dev)
-    a.K, a.k_batch, a.ldk = _long_rows("k", k, B, Sk, kv_heads * D, dt, dev)
-    a.V, a.v_batch, a.ldv = _long_rows("v", v, B, Sk, kv_heads * D, dt, dev)
-    for name, m, shape in (("key_mask", key_mask, (B, Sk)), ("key_count", key_count, (B,))):
-        if m is not None:
-            if m.dtype != torch.int32 or m.shape != shape or not m.is_contiguous() or m.device != dev:
-                raise ValueError(f"{name} must be a contiguous int32 {list(shape)} on {dev}")
-            setattr(a, name, m.data_ptr())
+    D = HD // heads
+    kv_shape = (B, Sk, kv_heads * D)
+    Q, qb, ldq = _rows("q", q, shape, dt, dev)
+    K, kb, ldk = _rows("k", k, kv_shape, dt, dev)
+    V, vb, ldv = _rows("v", v, kv_shape, dt, dev)
+    mask = count = table = buckets = nb = maxd = 0
+    if key_mask is not None:
+        if key_mask.dtype != torch.int32 or key_mask.shape != (B, Sk) or not key_mask.is_contiguous() or key_mask.device != dev:
+            raise ValueError(f"key_mask must be a contiguous int32 [{B}, {Sk}] on {dev}")
+        mask = key_mask.data_ptr()
+    if key_count is not None:
+        if key_count.dtype != torch.int32 or key_count.shape != (B,) or not key_count.is_contiguous() or key_count.device != dev:
+            raise ValueError(f"key_count must be a contiguous int32 [{B}] on {dev}")
+        count = key_count.data_ptr()
     if rel_bias is not None:
-        table, buckets = rel_bias
-        if table.dtype != dt or table.dim() != 2 or table.shape[1] != heads or not table.is_contiguous() or table.device != dev:
+        t, m = rel_bias
+        if t.dtype != dt or t.dim() != 2 or t.shape[1] != heads or not t.is_contiguous() or t.device != dev:
             raise ValueError(f"rel_bias = (table, buckets): the table must be a contiguous {dt} [num_buckets, {heads}] on {dev}")
-        a.max_distance = _check_buckets(buckets, dev)
-        a.table, a.buckets, a.num_buckets = table.data_ptr(), buckets.data_ptr(), table.shape[0]
-    if drop_p:
-        a.drop_p, a.seed, a.offset = drop_p, seed, offset
-    return a
+        maxd, nb, table, buckets = _check_buckets(m, dev), t.shape[0], t.data_ptr(), m.data_ptr()
+    if not 0.0 <= drop_p < 1.0:
+        raise ValueError(f"drop_p={drop_p} must be in [0, 1)")
+    if not drop_p:
+        seed = offset = 0
+    before = (B, heads, kv_heads, Sq, Sk, D, code, 1 if causal else 0, q_start, scale, mask, count, Q, K, V, 0, 0, 0, qb, kb, vb, ldq, ldk, ldv)
+    return before, (table, buckets, nb, maxd, drop_p, seed, offset)
+
+
+def _long_run(dev, what, fn, backward, fields):
+    a = _lib.LongAttnArgs.from_buffer_copy(_PACK(*fields, 0, 0))
+    nbytes = lib.didi_long_attention_workspace_bytes(a, backward)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _lib.check(_launch(dev, fn, a), what)
 
 
 def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_mask=None, key_count=None, scale=None, rel_bias=None, drop_p=0.0,
@@ -744,23 +779,18 @@ def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_
     gives zeros, and what lies at invisible keys is never used.  ``scale``: default 1/sqrt(D).  ``rel_bias`` = (table [num_buckets, heads],
     relative_buckets(...)): a learned bias by the distance from query q_start + i to the key, added to the scaled scores.  ``drop_p``,
     ``seed``, ``offset``: dropout of the probabilities, ``attention_train``'s mask.
-    ``need_grad``: -> (o, saved) for ``cross_attention_backward``.  ``out``: written in place (its strides as q's)."""
-    a = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
-    dev, B, Sq = q.device, a.B, a.Sq
-    with _on(dev):
-        o = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
-        a.O, a.o_batch, a.ldo = _long_rows("out", o, B, Sq, q.shape[2], q.dtype, dev)
-        saved = None
-        if need_grad:
-            # the output's remainder plane: the bias gradient's sums cancel and want D = do . o beyond o's own 8 or 11 bits
-            o_lo = torch.empty_strided(o.shape, o.stride(), dtype=q.dtype, device=dev) if rel_bias is not None and q.dtype != torch.float32 else None
-            saved = (torch.empty((B, heads, Sq), dtype=torch.float32, device=dev), o_lo)
-            a.lse, a.O_lo = saved[0].data_ptr(), _lib.ptr(o_lo)
-        nbytes = lib.didi_long_attention_workspace_bytes(a, 0)
-        if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        _lib.check(lib.didi_long_attention_forward(a, _lib.current_stream()), "cross_attention")
+    ``need_grad``: -> (o, saved) for ``cross_attention_backward``.  ``out``: written in place (views as for q)."""
+    before, after = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
+    dev, shape = q.device, q.shape
+    o = torch.empty(shape, dtype=q.dtype, device=dev) if out is None else out
+    O, ob, ldo = _rows("out", o, shape, q.dtype, dev)
+    saved, lse, lo = None, 0, 0
+    if need_grad:
+        # the output's remainder plane: the bias gradient's sums cancel and want D = do . o beyond o's own 8 or 11 bits
+        o_lo = torch.empty_strided(shape, o.stride(), dtype=q.dtype, device=dev) if rel_bias is not None and q.dtype != torch.float32 else None
+        saved = (torch.empty((shape[0], heads, shape[1]), dtype=torch.float32, device=dev), o_lo)
+        lse, lo = saved[0].data_ptr(), 0 if o_lo is None else o_lo.data_ptr()
+    _long_run(dev, "cross_attention", lib.didi_long_attention_forward, 0, (*before, O, lo, ob, ldo, lse, *after, *_NO_GRADS))
     return (o, saved) if need_grad else o
 
 
@@ -769,29 +799,26 @@ def cross_attention_backward(q, k, v, o, saved, dO, heads, kv_heads=None, causal
     """Backward of ``cross_attention(..., need_grad=True)`` with the same arguments -> (dq, dk, dv), and dtable where a bias was given.
     ``out`` = (dq, dk, dv): views to write into (e.g. the thirds of a fused projection's gradient); default fresh contiguous tensors.
     Deterministic."""
-    a = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
-    dev, dt, B, Sq, Sk = q.device, q.dtype, a.B, a.Sq, a.Sk
+    before, after = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
+    dev, dt, shape, kv_shape = q.device, q.dtype, q.shape, k.shape
     lse, o_lo = saved
-    if lse.shape != (B, heads, Sq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
+    if lse.shape != (shape[0], heads, shape[1]) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
         raise ValueError("saved must be what cross_attention returned for these operands")
-    with _on(dev):
-        a.O, a.o_batch, a.ldo = _long_rows("o", o, B, Sq, q.shape[2], dt, dev)
-        if o_lo is not None:
-            if o_lo.shape != o.shape or o_lo.stride() != o.stride():
-                raise ValueError("o must be the tensor (or a copy of its layout) that cross_attention returned")
-            a.O_lo = o_lo.data_ptr()
-        a.lse = lse.data_ptr()
-        a.dO, a.do_batch, a.lddo = _long_rows("dO", dO, B, Sq, q.shape[2], dt, dev)
-        grads = tuple(torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k, v)) if out is None else tuple(out)
-        a.dQ, a.dq_batch, a.lddq = _long_rows("dq", grads[0], B, Sq, q.shape[2], dt, dev)
-        a.dK, a.dk_batch, a.lddk = _long_rows("dk", grads[1], B, Sk, k.shape[2], dt, dev)
-        a.dV, a.dv_batch, a.lddv = _long_rows("dv", grads[2], B, Sk, k.shape[2], dt, dev)
-        if rel_bias is not None:
-            grads += (torch.empty_like(rel_bias[0]),)
-            a.dtable = grads[3].data_ptr()
-        nbytes = lib.didi_long_attention_workspace_bytes(a, 1)
-        if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        _lib.check(lib.didi_long_attention_backward(a, _lib.current_stream()), "cross_attention_backward")
+    if o_lo is not None and (o_lo.shape != shape or o_lo.stride() != o.stride()):
+        raise ValueError("o must be the tensor that cross_attention returned (or one laid out like it)")
+    O, ob, ldo = _rows("o", o, shape, dt, dev)
+    G, gb, ldg = _rows("dO", dO, shape, dt, dev)
+    if out is None:
+        grads = (torch.empty(shape, dtype=dt, device=dev), torch.empty(kv_shape, dtype=dt, device=dev), torch.empty(kv_shape, dtype=dt, device=dev))
+    else:
+        grads = tuple(out)
+    dq, dqb, lddq = _rows("dq", grads[0], shape, dt, dev)
+    dk, dkb, lddk = _rows("dk", grads[1], kv_shape, dt, dev)
+    dv, dvb, lddv = _rows("dv", grads[2], kv_shape, dt, dev)
+    dtable = 0
+    if rel_bias is not None:
+        grads += (torch.empty_like(rel_bias[0]),)
+        dtable = grads[3].data_ptr()
+    _long_run(dev, "cross_attention_backward", lib.didi_long_attention_backward, 1,
+              (*before, O, 0 if o_lo is None else o_lo.data_ptr(), ob, ldo, lse.data_ptr(), *after, G, gb, ldg, dq, dk, dv, dqb, dkb, dvb, lddq, lddk, lddv, dtable))
     return grads
