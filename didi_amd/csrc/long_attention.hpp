@@ -23,7 +23,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "common.hpp"
 #include "philox.hpp"
@@ -147,18 +146,31 @@ __device__ __forceinline__ void keep_order() {
     if constexpr (!T::F32) __builtin_amdgcn_sched_barrier(0);
 }
 
-// A operand for dot products over the head dim: lane = row row0 + (lane & 31) of the image, chunk 2 c + h
+// The lane number, made anew where it is asked for: the swizzled addresses that follow from it are then computed next to their reads (an
+// instruction each) instead of being kept in up to 64 registers across the loop.
+template <bool ANEW>
+__device__ __forceinline__ int lane_of(int lane) {
+    if constexpr (ANEW) asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// A operand for dot products over the head dim: lane = row row0 + (lane & 31) of the image, chunk 2 c + h.  16 bits: all chunks are read at once;
+// fp32: each when its products are issued (a product takes 64 cycles, about a read's latency: held all at once they only cost registers)
 template <class T, int DP>
 struct Rows {
-    static constexpr int N = DP / (2 * T::EPC);
-    uint4 x[N];
-    __device__ __forceinline__ void read(const char* img, int row0, int lane) {
-        constexpr int CH = DP / T::EPC;
-        const int row = lane & 31, h = lane >> 5;
-        img += row0 * CH * 16;  // row0 % 32 == 0: the swizzle repeats
+    static constexpr int N = DP / (2 * T::EPC), CH = DP / T::EPC;
+    uint4 x[T::F32 ? 1 : N];
+    const char* at;
+    int lane;
+    __device__ __forceinline__ void read(const char* img, int row0, int lane_) {
+        at = img + row0 * CH * 16;  // row0 % 32 == 0: the swizzle repeats
+        lane = lane_of<T::F32>(lane_);
+        if constexpr (!T::F32) {
 #pragma unroll
-        for (int c = 0; c < N; ++c) x[c] = *reinterpret_cast<const uint4*>(img + lds_off<CH>(row, 2 * c + h));
+            for (int c = 0; c < N; ++c) x[c] = chunk(c);
+        }
     }
+    __device__ __forceinline__ uint4 chunk(int c) const { return *reinterpret_cast<const uint4*>(at + lds_off<CH>(lane & 31, 2 * c + (lane >> 5))); }
 };
 
 // rows . frag -> [32 rows][32 lanes]
@@ -170,7 +182,7 @@ __device__ __forceinline__ f32x16 dot(const Rows<T, DP>& a, const Frag<T, DP>& f
 #pragma unroll
     for (int c = 0; c < Frag<T, DP>::N; ++c) {
         if constexpr (T::F32) {
-            const float4 af = __builtin_bit_cast(float4, a.x[c]), bf = __builtin_bit_cast(float4, f.x[c]);
+            const float4 af = __builtin_bit_cast(float4, a.chunk(c)), bf = __builtin_bit_cast(float4, f.x[c]);
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af.x, bf.x, acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af.y, bf.y, acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af.z, bf.z, acc, 0, 0, 0);
@@ -183,36 +195,32 @@ __device__ __forceinline__ f32x16 dot(const Rows<T, DP>& a, const Frag<T, DP>& f
 }
 
 // A operand for sums over 32 rows row0 .. of the image: lane = column, the rows in the order in which the lanes of a 32x32 result hold them.
-// 16 bits: transposing reads, fragment [16-row step][32 columns]; fp32: the column's 16 values of the lane's half, [columns][16]
+// 16 bits: transposing reads, fragment [16-row step][32 columns]; fp32: one value for each product, read when it is issued
 template <class T, int DP>
 struct Cols {
-    static constexpr int N = T::F32 ? DP / 32 * 16 : DP / 32 * 2;
-    using X = std::conditional_t<T::F32, float, uint4>;
-    X x[N];
-    __device__ __forceinline__ void read(const char* img, int row0, int lane) {
-        constexpr int CH = DP / T::EPC;
-        const int h = lane >> 5;
-        img += row0 * CH * 16;
-        if constexpr (T::F32) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) {
-                    const int row = 8 * (r >> 2) + 4 * h + (r & 3), d = dt * 32 + (lane & 31);
-                    x[dt * 16 + r] = *reinterpret_cast<const float*>(img + lds_off<CH>(row, d >> 2) + (d & 3) * 4);
-                }
-        } else {
-            const int i = lane & 15, dh = (lane >> 4) & 1;  // the lane's address in its 16 lanes' 4 x 16 block; which half of the 32 columns
+    static constexpr int CH = DP / T::EPC;
+    uint4 x[T::F32 ? 1 : DP / 32 * 2];
+    const char* at;
+    int lane;
+    __device__ __forceinline__ void read(const char* img, int row0, int lane_) {
+        at = img + row0 * CH * 16;
+        lane = lane_of<T::F32>(lane_);
+        if constexpr (!T::F32) {
+            const int h = lane >> 5, i = lane & 15, dh = (lane >> 4) & 1;  // the lane's address in its 16 lanes' 4 x 16 block; which half of the 32 columns
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int dt = 0; dt < DP / 32; ++dt) {
                     const int ra = 16 * s + 4 * h + (i >> 2), ch = dt * 4 + dh * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
-                    const uint2 lo = __builtin_bit_cast(uint2, tr_read(img + lds_off<CH>(ra, ch) + sub));
-                    const uint2 hi = __builtin_bit_cast(uint2, tr_read(img + lds_off<CH>(ra + 8, ch) + sub));
+                    const uint2 lo = __builtin_bit_cast(uint2, tr_read(at + lds_off<CH>(ra, ch) + sub));
+                    const uint2 hi = __builtin_bit_cast(uint2, tr_read(at + lds_off<CH>(ra + 8, ch) + sub));
                     x[s * (DP / 32) + dt] = make_uint4(lo.x, lo.y, hi.x, hi.y);
                 }
         }
+    }
+    __device__ __forceinline__ float value(int r, int dt) const {
+        const int row = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), d = dt * 32 + (lane & 31);
+        return *reinterpret_cast<const float*>(at + lds_off<CH>(row, d >> 2) + (d & 3) * 4);
     }
 };
 
@@ -232,7 +240,7 @@ __device__ __forceinline__ void add(const Cols<T, DP>& a, const f32x16& w, f32x1
 #pragma unroll
         for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[dt * 16 + r], w[r], acc[dt], 0, 0, 0);
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.value(r, dt), w[r], acc[dt], 0, 0, 0);
     } else {
         typedef float f2 __attribute__((ext_vector_type(2)));
         uint32_t pk[8];
@@ -763,7 +771,7 @@ struct BwdQCfg {
     static constexpr int BYTES = 2 * NS * IMG;
     static constexpr int JOIN = WK == 1 ? 0 : 4 * 32 * (DP + 4) * 4;
     static constexpr int LDS = BYTES > JOIN ? BYTES : JOIN;
-    static constexpr int WAVES = T::F32 ? (DP > 64 ? 1 : 2) : DP <= 64 && !BIAS ? 3 : 2;
+    static constexpr int WAVES = T::F32 ? (DP > 64 ? 1 : 2) : DP <= 64 && !BIAS ? 3 : DP > 96 && (BIAS || WK == 4) ? 1 : 2;
 };
 
 // Where the table's gradient is accumulated: one array of distances per wave, index d + maxd + PADB.  A 32x32 block's diagonals are summed through a
@@ -1116,7 +1124,7 @@ struct BwdKCfg {
     static constexpr int BYTES = NS * (2 * IMG + STAT);
     static constexpr int JOIN = WQ == 1 ? 0 : 4 * 32 * (DP + 4) * 4;
     static constexpr int LDS = BYTES > JOIN ? BYTES : JOIN;
-    static constexpr int WAVES = T::F32 || DP > 64 ? 1 : 2;
+    static constexpr int WAVES = DP > 64 ? 1 : 2;
 };
 
 template <class T, int DP, int WQ, bool BIAS>
