@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) la_bias_dense(const void* table, const in
 // changes are summed along their diagonals, one thread each (neighbouring threads read neighbouring columns); what lies left and right of
 // them goes, 16 bytes at a time, into two sums.  Bound by the one read of the gradient.
 template <class T>
-__global__ void __launch_bounds__(256) la_bias_grad(const void* dbias, LaParams p, int rows, int64_t total) {
+__global__ void __launch_bounds__(256) la_bias_grad(const void* dbias, LaParams p, int rows) {
     constexpr int EPC = T::EPC;
     extern __shared__ float sh[];  // 8 words for the range, 8 for the sums
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -96,64 +96,61 @@ __global__ void __launch_bounds__(256) la_bias_grad(const void* dbias, LaParams 
         float sum = 0.f;
         if (d >= lo && d <= hi) {
             const int a = max(i0, -d - p.q_start), z = min(i1, p.Sk - d - p.q_start);  // rows where 0 <= i + q_start + d < Sk
-#pragma unroll 8
+#pragma unroll 16
             for (int i = a; i < z; ++i) sum += T::elem(dbias, base + (int64_t)i * p.Sk + i + p.q_start + d);
         }
         out[x] = sum;
     }
+    // Two rows of a wave at a time, four 16-byte loads of each on their way.  A row's left part is cut from its first column on, its right part from
+    // jr on, wherever that lies in memory (the loads need no alignment); what is left over at the ends of the two parts is read element by element.
     float left = 0.f, right = 0.f;
-    for (int i = i0 + wave; i < i1; i += 4) {
-        const int64_t row = base + (int64_t)i * p.Sk;
-        const int jl = min(max(i + p.q_start + lo, 0), p.Sk), jr = min(max(i + p.q_start + hi + 1, 0), p.Sk);  // [0, jl) left, [jr, Sk) right
-        const int skew = (int)(row % EPC), chunks = (p.Sk + skew + EPC - 1) / EPC;  // chunk c: columns c EPC - skew ..
-        const int64_t first = row - skew;
-        for (int c0 = lane; c0 < chunks; c0 += 256) {  // four loads on their way together
-            uint4 x[4];
-            bool far[4];
+    const char* bytes = static_cast<const char*>(dbias);
+    for (int ia = i0 + wave; ia < i1; ia += 8) {
+        int64_t row[2];
+        int jl[2], jr[2], nl[2], n[2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int c = c0 + u * 64, j = c * EPC - skew;
-                far[u] = c < chunks && (j < jl || j + EPC > jr);
-                x[u] = make_uint4(0, 0, 0, 0);
-                if (!far[u]) continue;
-                if (first + (int64_t)(c + 1) * EPC <= total) {
-                    const void* at[2] = {dbias, nullptr};
-                    x[u] = T::load(at, first + (int64_t)c * EPC);
-                } else {  // the last elements of all
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    for (int e = 0; e < EPC; ++e)
-                        if (j + e < p.Sk) {
-                            if constexpr (T::F32) w[e] = static_cast<const uint32_t*>(dbias)[first + (int64_t)c * EPC + e];
-                            else w[e >> 1] |= (uint32_t)static_cast<const u16*>(dbias)[first + (int64_t)c * EPC + e] << (16 * (e & 1));
-                        }
-                    x[u] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int r = 0; r < 2; ++r) {
+            const int i = ia + 4 * r;
+            row[r] = base + (int64_t)i * p.Sk;
+            jl[r] = i < i1 ? min(max(i + p.q_start + lo, 0), p.Sk) : 0;
+            jr[r] = i < i1 ? min(max(i + p.q_start + hi + 1, 0), p.Sk) : p.Sk;  // [0, jl) left, [jr, Sk) right
+            nl[r] = jl[r] / EPC;
+            n[r] = nl[r] + (p.Sk - jr[r]) / EPC;
+        }
+        for (int c0 = lane; c0 < max(n[0], n[1]); c0 += 256) {
+            typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+            u4 x[2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int c = c0 + 64 * u;
+                    x[r][u] = u4{0, 0, 0, 0};
+                    if (c < n[r]) x[r][u] = *reinterpret_cast<const u4*>(bytes + (row[r] + (c < nl[r] ? c * EPC : jr[r] + (c - nl[r]) * EPC)) * T::ES);
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (!far[u]) continue;
-                const int j = (c0 + u * 64) * EPC - skew;
-                const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-                float v[EPC];
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-                for (int e = 0; e < EPC; ++e) {
-                    if constexpr (T::F32) v[e] = __builtin_bit_cast(float, w[e]);
-                    else v[e] = T::to_f32((u16)(w[e >> 1] >> (16 * (e & 1))));
-                }
-                if (j >= 0 && (j + EPC <= jl || (j >= jr && j + EPC <= p.Sk))) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int e = 0; e < EPC; ++e) sum += v[e];
-                    if (j < jl) left += sum;
-                    else right += sum;
-                } else {
+                for (int u = 0; u < 4; ++u) {
+                    float v[EPC];
 #pragma unroll
                     for (int e = 0; e < EPC; ++e) {
-                        if (j + e >= 0 && j + e < jl) left += v[e];
-                        if (j + e >= jr && j + e >= 0 && j + e < p.Sk) right += v[e];
+                        if constexpr (T::F32) v[e] = __builtin_bit_cast(float, (uint32_t)x[r][u][e]);
+                        else v[e] = T::to_f32((u16)(x[r][u][e >> 1] >> (16 * (e & 1))));
                     }
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < EPC; e += 4) sum += (v[e] + v[e + 1]) + (v[e + 2] + v[e + 3]);
+                    const bool is_left = c0 + 64 * u < nl[r];
+                    left += is_left ? sum : 0.f;
+                    right += is_left ? 0.f : sum;
                 }
-            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int tl = jl[r] % EPC, tr = (p.Sk - jr[r]) % EPC;
+            if (lane < tl) left += T::elem(dbias, row[r] + jl[r] - 1 - lane);
+            if (lane < tr) right += T::elem(dbias, row[r] + p.Sk - 1 - lane);
         }
     }
     left = wave_sum(left);
@@ -171,17 +168,20 @@ __global__ void __launch_bounds__(256) la_bias_grad(const void* dbias, LaParams 
 
 // ------------------------------------------------------------------ host side
 constexpr int MAX_DIST = 512, MAX_BUCKETS = 1024, MAX_SPLITS = 64;
-constexpr int64_t TARGET_WGS = 512;  // two workgroups on each of 256 CUs
 
 
-// groups: row groups (dialogs x heads); rows of each; n: length of the contraction; one: its tile at wk = 1 (32 wk otherwise); most: the largest wk
-Cut cut(int64_t groups, int64_t rows, int64_t n, int one, int most) {
+// groups: row groups (dialogs x heads); rows of each; n: length of the contraction; one: its tile at wk = 1 (32 wk otherwise); most: the largest wk.
+// wk = 1 from `full` workgroups on, 2 from `half` on, else 4 (us, 12 heads of 64 unless said): forward, 512 x 512 with a bias: 384 workgroups 20.3
+// (wk = 2: 18.4), 768: 25.9 (32.9); 16 heads of 128, 1024 x 1024: 128 workgroups 37.8, wk = 2 28.8, 4: 39.2; 63 x 512, 48 pairs: wk = 2 11.1,
+// 4 7.8.  More than one workgroup per block of rows costs a second launch and the partial sums' traffic: only where fewer than `target` would run,
+// and at least four tiles each (33000 keys, 12 pairs, one token: 199 us unsplit, 24 with 32 to 42; 512 keys, 12 pairs: 9.7 unsplit, 11.0 with 2).
+Cut cut(int64_t groups, int64_t rows, int64_t n, int one, int most, int64_t full, int64_t half, int64_t target) {
     Cut c{};
-    c.wk = rows <= 32 || groups * cdiv(rows, 64) < 256 ? 4 : groups * cdiv(rows, 128) < 256 ? 2 : 1;
+    c.wk = rows <= 32 || groups * cdiv(rows, 64) < half ? 4 : groups * cdiv(rows, 128) < full ? 2 : 1;
     c.wk = std::min(c.wk, most);
     c.nrt = cdiv(rows, 128 / c.wk);
     const int64_t base = std::max<int64_t>(1, groups * c.nrt), tile = c.wk == 1 ? one : 32 * c.wk, tiles = std::max<int64_t>(1, (n + tile - 1) / tile);
-    c.ns = (int)std::max<int64_t>(1, std::min<int64_t>({TARGET_WGS / base, tiles / 4, (int64_t)MAX_SPLITS}));
+    c.ns = (int)std::max<int64_t>(1, std::min<int64_t>({target / base, tiles / 4, (int64_t)MAX_SPLITS}));
     c.per = (int)((tiles + c.ns - 1) / c.ns);
     return c;
 }
@@ -191,12 +191,15 @@ Plan make_plan(const didi_long_attn_args* a) {
     const bool f32 = a->dtype == DIDI_DT_FP32 || a->Q_lo;
     const int G = a->heads / a->kv_heads, one = f32 ? 32 : 64, most = max_share(f32, pad_dim(a->D));
     const int64_t HG = a->table ? a->heads : a->kv_heads, R = (int64_t)(a->table ? 1 : G) * a->Sq, rows = (int64_t)a->B * a->heads * a->Sq;
-    z.f = cut(a->B * HG, R, a->Sk, one, most);
+    // one token per row group: the keys are all there is to read, and dialogs of different lengths want smaller pieces (32 dialogs to 4096 keys:
+    // 50.5 us unsplit, 45.6 to 47.4 with 2 to 4)
+    const bool few = R <= 32;
+    z.f = cut(a->B * HG, R, a->Sk, one, most, 512, 192, !few ? 256 : a->B * HG > 256 ? 1152 : 512);
     int most_q = most;  // wide biases: the sums by distance take the room of shared tiles
     if (a->table)
         while (most_q > 1 && 2 * stages(image_bytes(f32, pad_dim(a->D), most_q)) * image_bytes(f32, pad_dim(a->D), most_q) + sums_lds(a->max_distance) > MAX_LDS) most_q /= 2;
-    z.q = cut(a->B * HG, R, a->Sk, one, most_q);
-    z.k = cut((int64_t)a->B * a->kv_heads, a->Sk, (int64_t)G * a->Sq, one, most);
+    z.q = cut(a->B * HG, R, a->Sk, one, most_q, 256, 192, 256);
+    z.k = cut((int64_t)a->B * a->kv_heads, a->Sk, (int64_t)G * a->Sq, one, most, 128, 128, 128);  // 15 x 777 keys of 80: wk = 1 41.8 us, 2 40.5, 4 46.8 (of the whole backward)
     {  // the contraction of la_backward_kv is counted in tiles of each head
         const int64_t tile = z.k.wk == 1 ? one : 32 * z.k.wk, tiles = std::max<int64_t>(1, G * ((a->Sq + tile - 1) / tile));
         z.k.per = (int)((tiles + z.k.ns - 1) / z.k.ns);
@@ -376,8 +379,7 @@ extern "C" int didi_relative_bias_backward(const void* dbias, const int32_t* buc
         const int rows = grad_rows((int64_t)B * heads, Sq);
         parts = cdiv(Sq, rows);
         const dim3 grid(parts, B * heads);
-        const int64_t total = (int64_t)B * heads * Sq * Sk;
-#define DIDI_GRAD(T) la_bias_grad<T><<<grid, 256, 16 * 4, st>>>(dbias, p, rows, total)
+#define DIDI_GRAD(T) la_bias_grad<T><<<grid, 256, 16 * 4, st>>>(dbias, p, rows)
         if (dtype == DIDI_DT_FP32) DIDI_GRAD(EF32);
         else if (dtype == DIDI_DT_FP16) DIDI_GRAD(E16<true>);
         else DIDI_GRAD(E16<false>);

@@ -1059,14 +1059,14 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
 template <class T>
 __global__ void __launch_bounds__(1024) la_table_sum(const float* tpart, const int32_t* map, int B, int H, int parts, int nb, int maxd, void* out) {
     extern __shared__ float dist[];  // [4][nd + 2], then the map
-    const int h = blockIdx.x, nd = 2 * maxd + 1, n = nd + 2, tid = threadIdx.x, grp = tid >> 8, total = B * parts;
+    const int h = blockIdx.x, nd = 2 * maxd + 1, n = nd + 2, tid = threadIdx.x, grp = tid >> 8;
     for (int x = tid; x < nd; x += 1024) reinterpret_cast<int*>(dist + 4 * n)[x] = map[x];
     for (int x = tid & 255; x < n; x += 256) {
         float sum = 0.f;
+        for (int b = 0; b < B; ++b) {
+            const float* at = tpart + ((int64_t)b * H + h) * parts * n + x;
 #pragma unroll 16
-        for (int k = grp; k < total; k += 4) {
-            const int b = k / parts;
-            sum += tpart[(((int64_t)b * H + h) * parts + (k - b * parts)) * n + x];
+            for (int k = grp; k < parts; k += 4) sum += at[(int64_t)k * n];
         }
         dist[grp * n + x] = sum;
     }
