@@ -175,13 +175,14 @@ struct Rows {
 
 // rows . frag -> [32 rows][32 lanes]
 template <class T, int DP>
-__device__ __forceinline__ f32x16 dot(const Rows<T, DP>& a, const Frag<T, DP>& f) {
+__device__ __forceinline__ f32x16 dot(const Rows<T, DP>& a, const Frag<T, DP>& f, int D) {
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int c = 0; c < Frag<T, DP>::N; ++c) {
         if constexpr (T::F32) {
+            if (c > 0 && c * 2 * T::EPC >= D) break;  // 256 cycles each: columns of padding are left out
             const float4 af = __builtin_bit_cast(float4, a.chunk(c)), bf = __builtin_bit_cast(float4, f.x[c]);
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af.x, bf.x, acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af.y, bf.y, acc, 0, 0, 0);
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
             Rows<T, DP> ak;
             ak.read(Ks, krow, lane);
             keep_order<T>();
-            f32x16 s = dot<T, DP>(ak, q);
+            f32x16 s = dot<T, DP>(ak, q, p.D);
             Cols<T, DP> cv;  // the values are on their way while the softmax is computed
             cv.read(Vs, krow, lane);
             keep_order<T>();
@@ -921,11 +922,11 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
                 Rows<T, DP> a;
                 a.read(Ks, krow + nt * 32, lane);
                 keep_order<T>();
-                f32x16 s = dot<T, DP>(a, q);
+                f32x16 s = dot<T, DP>(a, q, p.D);
                 keep_order<T>();
                 a.read(Vs, krow + nt * 32, lane);
                 keep_order<T>();
-                f32x16 dp = dot<T, DP>(a, go);
+                f32x16 dp = dot<T, DP>(a, go, p.D);
                 if (near) {
                     asm volatile("");
 #pragma unroll
@@ -1213,18 +1214,18 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
             for (int nt = 0; nt < C::NT; ++nt) {
                 const int i1 = i0 + qrow + nt * 32;
                 Rows<T, DP> a;
+                Cols<T, DP> c;
                 a.read(Qs, qrow + nt * 32, lane);
                 keep_order<T>();
-                f32x16 s = dot<T, DP>(a, kf);
+                f32x16 s = dot<T, DP>(a, kf, p.D);
                 keep_order<T>();
                 a.read(Gs, qrow + nt * 32, lane);
-                keep_order<T>();
-                f32x16 dp = dot<T, DP>(a, vf);
+                c.read(Gs, qrow + nt * 32, lane);
                 const int p0 = p.q_start + i1, dmin = kw - p0 - 31, dmax = kw + 31 - p0;
                 const bool near = BIAS && dmax >= blo && dmin <= bhi;
                 const float fc = vis ? (BIAS ? (dmax < blo ? bv[0] : bv[len - 1]) : 0.f) : -INFINITY;
                 const int at = key - p0 + p.maxd + PADB - 4 * h;
-                float ls[16];
+                float ls[16];  // -lse log2(e) of the lane's rows, then with the bias
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {
                     const float4 l4 = *reinterpret_cast<const float4*>(rc + nt * 32 + 8 * gq + 4 * h);
@@ -1241,8 +1242,21 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
 #pragma unroll
                     for (int e = 0; e < 16; ++e) ls[e] += fc;
                 }
+                // a wave issues in order and a product that waits for the one before it holds everything behind it up: the exponentials go between
+                // the products of do . v, the score gradients between those of dV
+                keep_order<T>();
+                f32x16 dp = dot<T, DP>(a, vf, p.D);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.sc, ls[e]));
+                if constexpr (!T::F32) {
+#pragma unroll
+                    for (int x = 0; x < DP / 16; ++x) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 256 / DP, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 256 / DP, 0);
+                    }
+                }
+                keep_order<T>();
                 if (p.causal && kw + 31 > p0) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
@@ -1253,7 +1267,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
                     for (int e = 0; e < 16; ++e)
                         if (i1 + 8 * (e >> 2) + 4 * h + (e & 3) >= p.Sq) s[e] = 0.f;
                 }
-                f32x16 ds;
+                f32x16 pd = s;  // the probabilities behind the dropout
                 if (p.thr) {
                     asm volatile("");  // a branch: speculated, the random numbers would cost more than all the rest
                     const int t4 = lane & 3;
@@ -1264,41 +1278,45 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
                         const int i = i1 + 8 * gq + 4 * h + t4;
                         float k[4];
                         drop4(p, ((uint64_t)b * p.H + head) * p.Sq + i, key & ~3, k);
-                        float mk[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int src = (lane & ~3) | e;
                             const float w0 = __shfl(k[0], src, 64), w1 = __shfl(k[1], src, 64), w2 = __shfl(k[2], src, 64), w3 = __shfl(k[3], src, 64);
-                            mk[e] = t4 == 0 ? w0 : t4 == 1 ? w1 : t4 == 2 ? w2 : w3;
-                        }
-                        const float4 d4 = *reinterpret_cast<const float4*>(rc + 64 + nt * 32 + 8 * gq + 4 * h);
-                        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            ds[4 * gq + e] = s[4 * gq + e] * fmaf(dp[4 * gq + e], mk[e], -dl[e]);
-                            s[4 * gq + e] *= mk[e];
+                            const float mk = t4 == 0 ? w0 : t4 == 1 ? w1 : t4 == 2 ? w2 : w3;
+                            pd[4 * gq + e] *= mk;
+                            dp[4 * gq + e] *= mk;
                         }
                     }
-                } else {
+                }
+                Cols<T, DP> cq;
+                cq.read(Qs, qrow + nt * 32, lane);
+                float dl[16];
 #pragma unroll
-                    for (int gq = 0; gq < 4; ++gq) {
-                        const float4 d4 = *reinterpret_cast<const float4*>(rc + 64 + nt * 32 + 8 * gq + 4 * h);
-                        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
+                for (int gq = 0; gq < 4; ++gq) {
+                    const float4 d4 = *reinterpret_cast<const float4*>(rc + 64 + nt * 32 + 8 * gq + 4 * h);
+                    dl[4 * gq] = d4.x;
+                    dl[4 * gq + 1] = d4.y;
+                    dl[4 * gq + 2] = d4.z;
+                    dl[4 * gq + 3] = d4.w;
+                }
+                keep_order<T>();
+                add<T, DP>(c, pd, dv);
+                f32x16 ds;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) ds[4 * gq + e] = s[4 * gq + e] * (dp[4 * gq + e] - dl[e]);
+                for (int e = 0; e < 16; ++e) {
+                    ds[e] = s[e] * (dp[e] - dl[e]);
+                    if constexpr (T::F16) ds[e] *= fs;
+                }
+                if constexpr (!T::F32) {
+                    __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);  // the probabilities' roundings
+#pragma unroll
+                    for (int x = 0; x < DP / 16; ++x) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 768 / DP, 0);
                     }
                 }
-                if constexpr (T::F16) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) ds[e] *= fs;
-                }
                 keep_order<T>();
-                Cols<T, DP> c;
-                c.read(Gs, qrow + nt * 32, lane);
-                add<T, DP>(c, s, dv);
-                keep_order<T>();
-                c.read(Qs, qrow + nt * 32, lane);
-                add<T, DP>(c, ds, dk);
+                add<T, DP>(cq, ds, dk);
             }
         }
     }
