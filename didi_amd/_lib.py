@@ -82,7 +82,7 @@ class LongAttnArgs(C.Structure):
         ("B", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("Sq", C.c_int), ("Sk", C.c_int), ("D", C.c_int),
         ("dtype", C.c_int), ("causal", C.c_int), ("q_start", C.c_int), ("scale", C.c_float),
         ("key_mask", C.c_void_p), ("key_count", C.c_void_p),
-        ("Q", C.c_void_p), ("K", C.c_void_p), ("V", C.c_void_p), ("Q_lo", C.c_void_p), ("K_lo", C.c_void_p), ("V_lo", C.c_void_p),
+        ("Q", C.c_void_p), ("K", C.c_void_p), ("V", C.c_void_p),
         ("q_batch", C.c_int64), ("k_batch", C.c_int64), ("v_batch", C.c_int64), ("ldq", C.c_int), ("ldk", C.c_int), ("ldv", C.c_int),
         ("O", C.c_void_p), ("O_lo", C.c_void_p), ("o_batch", C.c_int64), ("ldo", C.c_int), ("lse", C.c_void_p),
         ("table", C.c_void_p), ("buckets", C.c_void_p), ("num_buckets", C.c_int), ("max_distance", C.c_int),

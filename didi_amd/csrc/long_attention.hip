@@ -188,7 +188,7 @@ Cut cut(int64_t groups, int64_t rows, int64_t n, int one, int most, int64_t full
 
 Plan make_plan(const didi_long_attn_args* a) {
     Plan z{};
-    const bool f32 = a->dtype == DIDI_DT_FP32 || a->Q_lo;
+    const bool f32 = a->dtype == DIDI_DT_FP32;
     const int G = a->heads / a->kv_heads, one = f32 ? 32 : 64, most = max_share(f32, pad_dim(a->D));
     const int64_t HG = a->table ? a->heads : a->kv_heads, R = (int64_t)(a->table ? 1 : G) * a->Sq, rows = (int64_t)a->B * a->heads * a->Sq;
     // one token per row group: the keys are all there is to read, and dialogs of different lengths want smaller pieces (32 dialogs to 4096 keys:
@@ -221,10 +221,9 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
     DIDI_CHECK_ARG(a && a->B >= 0 && a->Sq >= 0 && a->Sk >= 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->D > 0);
     DIDI_CHECK_ARG(a->dtype == DIDI_DT_BF16 || a->dtype == DIDI_DT_FP16 || a->dtype == DIDI_DT_FP32);
     DIDI_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && a->drop_p >= 0.f && a->drop_p < 1.f && a->q_start >= 0);
-    const bool planes = a->Q_lo || a->K_lo || a->V_lo, f32 = a->dtype == DIDI_DT_FP32;
-    if (planes) DIDI_CHECK_ARG(!f32 && (a->Q_lo || !a->Q) && (a->K_lo || !a->K) && (a->V_lo || !a->V) && !bwd && !a->table);
+    const bool f32 = a->dtype == DIDI_DT_FP32;
     DIDI_CHECK_ARG(!(f32 && a->O_lo));
-    if (a->D > 128 || a->D % (f32 || planes ? 4 : 8) != 0) return DIDI_ERR_UNSUPPORTED;
+    if (a->D > 128 || a->D % (f32 ? 4 : 8) != 0) return DIDI_ERR_UNSUPPORTED;
     if (a->table) {
         DIDI_CHECK_ARG(a->buckets && a->num_buckets > 0 && a->max_distance > 0);
         if (a->max_distance > MAX_DIST || a->num_buckets > MAX_BUCKETS) return DIDI_ERR_UNSUPPORTED;
@@ -236,7 +235,7 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
         if (ld > (1 << 21)) return DIDI_ERR_UNSUPPORTED;
     if ((int64_t)a->Sq * a->heads > lim || cdiv((int64_t)a->Sq * a->heads, 32) > 65535 || cdiv(a->Sk, 32) > 65535 || a->Sk > lim || (int64_t)a->q_start + a->Sq > lim || (int64_t)a->B * a->heads > (1 << 20)) return DIDI_ERR_UNSUPPORTED;
     const int64_t wq = (int64_t)a->heads * a->D, wk = (int64_t)a->kv_heads * a->D;
-    const int e = f32 ? 4 : 2, al = planes ? 8 : 16;
+    const int e = f32 ? 4 : 2;
     struct Op {
         const void* p;
         int64_t batch;
@@ -246,17 +245,16 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
     } ops[] = {
         {a->Q, a->q_batch, a->ldq, a->Sq, wq, true, false},   {a->K, a->k_batch, a->ldk, a->Sk, wk, true, false},
         {a->V, a->v_batch, a->ldv, a->Sk, wk, true, false},   {a->O, a->o_batch, a->ldo, a->Sq, wq, true, !bwd},
-        {a->Q_lo, a->q_batch, a->ldq, a->Sq, wq, false, false}, {a->K_lo, a->k_batch, a->ldk, a->Sk, wk, false, false},
-        {a->V_lo, a->v_batch, a->ldv, a->Sk, wk, false, false}, {a->O_lo, a->o_batch, a->ldo, a->Sq, wq, false, !bwd},
+        {a->O_lo, a->o_batch, a->ldo, a->Sq, wq, false, !bwd},
         {a->dO, a->do_batch, a->lddo, a->Sq, wq, bwd, false}, {a->dQ, a->dq_batch, a->lddq, a->Sq, wq, bwd, true},
         {a->dK, a->dk_batch, a->lddk, a->Sk, wk, bwd, true},  {a->dV, a->dv_batch, a->lddv, a->Sk, wk, bwd, true},
     };
     for (const Op& o : ops) {
-        if (a->B == 0 || o.S == 0 || (!bwd && &o >= ops + 8)) continue;  // the forward does not look at the gradients' fields
+        if (a->B == 0 || o.S == 0 || (!bwd && &o >= ops + 5)) continue;  // the forward does not look at the gradients' fields
         if (o.need) DIDI_CHECK_ARG(o.p);
         if (!o.p) continue;
         DIDI_CHECK_ARG(o.ld >= o.w || o.S == 1);
-        DIDI_CHECK_ARG(o.batch >= 0 && aligned(o.p, o.batch, o.ld, al, e));
+        DIDI_CHECK_ARG(o.batch >= 0 && aligned(o.p, o.batch, o.ld, 16, e));
         if (o.written && a->B > 1) DIDI_CHECK_ARG(o.batch >= (int64_t)(o.S - 1) * o.ld + o.w);  // dialogs of an output may not overlap
     }
     DIDI_CHECK_ARG(!bwd || a->lse || a->B == 0 || a->Sq == 0);
@@ -272,7 +270,7 @@ LaParams make_params(const didi_long_attn_args* a) {
     p.scale = a->scale > 0.f ? a->scale : 1.0f / sqrtf((float)a->D);
     p.sc = p.scale * LOG2E;
     p.mask = a->key_mask; p.count = a->key_count;
-    p.Q[0] = a->Q; p.Q[1] = a->Q_lo; p.K[0] = a->K; p.K[1] = a->K_lo; p.V[0] = a->V; p.V[1] = a->V_lo;
+    p.Q = a->Q; p.K = a->K; p.V = a->V;
     p.dO = a->dO; p.O[0] = a->O; p.O[1] = a->O_lo; p.Ow[0] = a->O; p.Ow[1] = a->O_lo;
     p.dQ = a->dQ; p.dK = a->dK; p.dV = a->dV;
     p.qb = a->q_batch; p.kb = a->k_batch; p.vb = a->v_batch; p.ob = a->o_batch; p.dob = a->do_batch;
@@ -306,7 +304,6 @@ extern "C" int didi_long_attention_forward(const didi_long_attn_args* a, void* s
     p.part = static_cast<float*>(a->workspace);
     p.ml = p.part + (int64_t)q.f.ns * a->B * a->heads * a->Sq * a->D;
     hipStream_t st = as_stream(stream);
-    if (a->Q_lo) return forward_planes(p, q.f, a->dtype == DIDI_DT_FP16, st);
     if (a->dtype == DIDI_DT_FP32) return forward_fp32(p, q.f, st);
     return a->dtype == DIDI_DT_FP16 ? forward_fp16(p, q.f, st) : forward_bf16(p, q.f, st);
 }

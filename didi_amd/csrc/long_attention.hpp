@@ -41,7 +41,7 @@ struct LaParams {
     int causal, q_start;
     float scale, sc;  // sc = scale * log2(e): the softmax runs in base 2
     const int32_t *mask, *count;
-    const void *Q[2], *K[2], *V[2], *dO, *O[2];
+    const void *Q, *K, *V, *dO, *O[2];
     void *Ow[2], *dQ, *dK, *dV;
     int64_t qb, kb, vb, ob, dob, dqb, dkb, dvb;  // elements between dialogs
     int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
@@ -61,9 +61,9 @@ struct LaParams {
 // ---- element types: how operands lie in memory, what multiplies them
 template <bool F16_>
 struct E16 {
-    static constexpr bool F32 = false, F16 = F16_, ASYNC = true;
+    static constexpr bool F32 = false, F16 = F16_;
     static constexpr int ES = 2, EPC = 8;  // elements per 16-byte LDS chunk
-    __device__ static uint4 load(const void* const* p, int64_t off) { return *reinterpret_cast<const uint4*>(static_cast<const u16*>(p[0]) + off); }
+    __device__ static uint4 load(const void* p, int64_t off) { return *reinterpret_cast<const uint4*>(static_cast<const u16*>(p) + off); }
     __device__ static float to_f32(u16 x) { return F16 ? f16_to_f32(x) : bf16_to_f32(x); }
     __device__ static void store4(void* const* p, int64_t off, const float v[4]) {
         uint2 hi, lo;
@@ -74,30 +74,14 @@ struct E16 {
     __device__ static float elem(const void* p, int64_t off) { return to_f32(static_cast<const u16*>(p)[off]); }
 };
 struct EF32 {
-    static constexpr bool F32 = true, F16 = false, ASYNC = true;
+    static constexpr bool F32 = true, F16 = false;
     static constexpr int ES = 4, EPC = 4;
-    __device__ static uint4 load(const void* const* p, int64_t off) { return *reinterpret_cast<const uint4*>(static_cast<const float*>(p[0]) + off); }
+    __device__ static uint4 load(const void* p, int64_t off) { return *reinterpret_cast<const uint4*>(static_cast<const float*>(p) + off); }
     __device__ static void store4(void* const* p, int64_t off, const float v[4]) {
         *reinterpret_cast<float4*>(static_cast<float*>(p[0]) + off) = make_float4(v[0], v[1], v[2], v[3]);
     }
     __device__ static float elem(const void* p, int64_t off) { return static_cast<const float*>(p)[off]; }
 };
-// fp32 arithmetic on split planes (value = hi + lo), results as planes
-template <bool F16_>
-struct EPlanes {
-    static constexpr bool F32 = true, F16 = F16_, ASYNC = false;
-    static constexpr int ES = 2, EPC = 4;
-    __device__ static uint4 load(const void* const* p, int64_t off) {
-        float a[4], b[4];
-        unpack4(*reinterpret_cast<const uint2*>(static_cast<const u16*>(p[0]) + off), a, F16);
-        unpack4(*reinterpret_cast<const uint2*>(static_cast<const u16*>(p[1]) + off), b, F16);
-        const float4 s = make_float4(a[0] + b[0], a[1] + b[1], a[2] + b[2], a[3] + b[3]);
-        return __builtin_bit_cast(uint4, s);
-    }
-    __device__ static void store4(void* const* p, int64_t off, const float v[4]) { E16<F16_>::store4(p, off, v); }
-    __device__ static float elem(const void* p, int64_t off) { return static_cast<const float*>(p)[off]; }
-};
-
 // ---- LDS images [rows][DP] in 16-byte chunks, XOR-swizzled within a row so that the reads use all 64 banks: 16 neighbouring rows at one chunk
 // (MFMA A rows) fall into 16 different chunks of 256 bytes, and 4 neighbouring rows at 4 neighbouring chunks (what 32 lanes of a transposing
 // read fetch) into 4 different quarters.  With the rows' low bits alone a transposing read took two turns.
@@ -123,7 +107,7 @@ template <class T, int DP>
 struct Frag {
     static constexpr int N = DP / (2 * T::EPC);
     uint4 x[N];
-    __device__ void load(const void* const* p, int64_t off, bool ok, int D, int h) {
+    __device__ void load(const void* p, int64_t off, bool ok, int D, int h) {
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             const int col = (2 * c + h) * T::EPC;
@@ -314,31 +298,19 @@ struct Tile {
         }
     }
     // base: element offset of the tile's first row; n: rows of it that exist; masked: bit r of word r / 64 of keep
-    __device__ __forceinline__ void copy(const void* const* p, int64_t base, int64_t ld, int n, bool masked, const uint64_t* keep, int keep_shift, char* smem,
+    __device__ __forceinline__ void copy(const void* p, int64_t base, int64_t ld, int n, bool masked, const uint64_t* keep, int keep_shift, char* smem,
                                          uint32_t img, int tid) const {
-        if constexpr (T::ASYNC) {
-            const i32x4 rs = resource(static_cast<const char*>(p[0]) + base * T::ES, (uint32_t)max(min(n, ROWS), 0) * (uint32_t)(ld * T::ES));
-            const uint32_t dst = (uint32_t)(uintptr_t)(lds_void*)smem + img + (tid >> 6) * 1024;
-            if (masked) {
+        const i32x4 rs = resource(static_cast<const char*>(p) + base * T::ES, (uint32_t)max(min(n, ROWS), 0) * (uint32_t)(ld * T::ES));
+        const uint32_t dst = (uint32_t)(uintptr_t)(lds_void*)smem + img + (tid >> 6) * 1024;
+        if (masked) {
 #pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    const int r = row(j, tid) + keep_shift;
-                    copy16((keep[r >> 6] >> (r & 63)) & 1 ? off[j] : NOWHERE, rs, dst + j * 4096);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < NC; ++j) copy16(off[j], rs, dst + j * 4096);
+            for (int j = 0; j < NC; ++j) {
+                const int r = row(j, tid) + keep_shift;
+                copy16((keep[r >> 6] >> (r & 63)) & 1 ? off[j] : NOWHERE, rs, dst + j * 4096);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                const int r = row(j, tid);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                bool ok = r < n && off[j] != NOWHERE;
-                if (masked) ok = ok && ((keep[(r + keep_shift) >> 6] >> ((r + keep_shift) & 63)) & 1);
-                if (ok) x = T::load(p, base + off[j] / T::ES);
-                *reinterpret_cast<uint4*>(smem + img + (tid + j * 256) * 16) = x;
-            }
+            for (int j = 0; j < NC; ++j) copy16(off[j], rs, dst + j * 4096);
         }
     }
 };
@@ -549,10 +521,9 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
 
     int cur = 0;
     for (int t = t0; t < t1; ++t) {
-        if constexpr (T::ASYNC) {  // this tile has landed; the later ones may be on their way
-            if (C::NS > 2 && t + 1 < t1) wait_copies<(C::NS > 2 ? 1 : 0) * 2 * KV::NC>();
-            else wait_copies<0>();
-        }
+        // this tile has landed; the later ones may be on their way
+        if (C::NS > 2 && t + 1 < t1) wait_copies<(C::NS > 2 ? 1 : 0) * 2 * KV::NC>();
+        else wait_copies<0>();
         barrier();
         keys.advance(t * C::BN, tid);
         if (t + C::NS - 1 < t1) issue(t + C::NS - 1);
@@ -824,13 +795,12 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
 
     Frag<T, DP> q, go;
     q.load(p.Q, (int64_t)b * p.qb + (int64_t)i * p.ldq + head * p.D, rok, p.D, h);
-    const void* dop[2] = {p.dO, nullptr};
-    go.load(dop, (int64_t)b * p.dob + (int64_t)i * p.lddo + head * p.D, rok, p.D, h);
+    go.load(p.dO, (int64_t)b * p.dob + (int64_t)i * p.lddo + head * p.D, rok, p.D, h);
     float delta = 0.f, norm = 0.f;
     {
         const int64_t oo = (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D;
         Frag<T, DP> o;
-        o.load(p.O, oo, rok, p.D, h);
+        o.load(p.O[0], oo, rok, p.D, h);
 #pragma unroll
         for (int c = 0; c < Frag<T, DP>::N; ++c) {
             if constexpr (T::F32) {
@@ -848,8 +818,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
         }
         if constexpr (!T::F32) {
             if (p.O[1]) {  // the output's remainder: the sums of ds by distance cancel, so D wants more than the output's 8 or 11 bits
-                const void* lo[2] = {p.O[1], nullptr};
-                o.load(lo, oo, rok, p.D, h);
+                o.load(p.O[1], oo, rok, p.D, h);
 #pragma unroll
                 for (int c = 0; c < Frag<T, DP>::N; ++c) {
                     const uint32_t a[4] = {o.x[c].x, o.x[c].y, o.x[c].z, o.x[c].w}, e[4] = {go.x[c].x, go.x[c].y, go.x[c].z, go.x[c].w};
@@ -1149,12 +1118,11 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     QT tq, tg;
     tq.init(p.ldq, p.D, tid);
     tg.init(p.lddo, p.D, tid);
-    const void* dop[2] = {p.dO, nullptr};
     auto issue = [&](int t) {
         const int head = kvh * p.G + t / nq, i0 = (qt0 + t % nq) * C::BQ;
         const uint32_t img = (t - t0) % C::NS * (2 * C::IMG + C::STAT);
         tq.copy(p.Q, (int64_t)b * p.qb + (int64_t)i0 * p.ldq + head * p.D, p.ldq, p.Sq - i0, false, nullptr, 0, smem, img, tid);
-        tg.copy(dop, (int64_t)b * p.dob + (int64_t)i0 * p.lddo + head * p.D, p.lddo, p.Sq - i0, false, nullptr, 0, smem, img + C::IMG, tid);
+        tg.copy(p.dO, (int64_t)b * p.dob + (int64_t)i0 * p.lddo + head * p.D, p.lddo, p.Sq - i0, false, nullptr, 0, smem, img + C::IMG, tid);
         const int i1 = i0 + wq * 32 * C::NT;  // this wave's rows
         const int64_t rowid = ((int64_t)b * p.H + head) * p.Sq + i1;
         const uint32_t st = (uint32_t)(uintptr_t)(lds_void*)smem + img + 2 * C::IMG + wave * 512;
@@ -1513,11 +1481,10 @@ int run_backward_t(const LaParams& p, const Plan& z, void* dtable, hipStream_t s
     }
 }
 
-// one definition of each per unit: long_attention_{bf16,fp16,fp32}_{forward,backward}.hip, long_attention_planes.hip
+// one definition of each per unit: long_attention_{bf16,fp16,fp32}_{forward,backward}.hip
 int forward_bf16(const LaParams& p, const Cut& c, hipStream_t st);
 int forward_fp16(const LaParams& p, const Cut& c, hipStream_t st);
 int forward_fp32(const LaParams& p, const Cut& c, hipStream_t st);
-int forward_planes(const LaParams& p, const Cut& c, bool f16, hipStream_t st);
 int backward_bf16(const LaParams& p, const Plan& z, void* dtable, hipStream_t st);
 int backward_fp16(const LaParams& p, const Plan& z, void* dtable, hipStream_t st);
 int backward_fp32(const LaParams& p, const Plan& z, void* dtable, hipStream_t st);

@@ -336,10 +336,17 @@ class DiDiSampler:
         E, A = cfg.enc_dim, cfg.enc_heads
         mask32 = attention_mask.to(torch.int32).contiguous()
 
+        if cfg.enc_kind != "t5" and Cn > e["pos"].shape[0]:
+            raise ValueError(f"a context of {Cn} tokens: the encoder has {e['pos'].shape[0]} positions")
+
+        long = Cn > ops.ATTENTION_MAX_LEN  # past the lengths the attention kernels of a dialog are built for: fp32 attention of any length
         wide_heads = E // A > 64 or (E // A) % 8 != 0  # e.g. Blenderbot-3B's 80-wide heads (configs/train.yaml:3)
 
         def attn(qkv_hi, qkv_lo, qkv_f32=None):
             v = lambda t, i: None if t is None else t.view(B, Cn, 3 * E)[:, :, i * E:(i + 1) * E]  # noqa: E731
+            if long:
+                o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32)
+                return ops.split(o.view(B * Cn, E))
             if wide_heads:  # past the MFMA attention kernel's head dim: the fp32 LDS kernel of the training forward (cold path)
                 o = ops.attention_train(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, causal=False, key_mask=mask32)
                 return ops.split(o.view(B * Cn, E))
@@ -352,7 +359,7 @@ class DiDiSampler:
             h = ops.embed_gather(input_ids, e["tok"], scale, e["pos"]).view(B * Cn, E)
             for ly in e["layers"]:
                 y_hi, y_lo, _ = ops.layernorm(h, *ly["ln1"], cfg.enc_ln_eps)
-                qkv_hi, qkv_lo, qkv32 = ly["qkv"](y_hi, y_lo, P, out_f32=wide_heads)
+                qkv_hi, qkv_lo, qkv32 = ly["qkv"](y_hi, y_lo, P, out_f32=wide_heads or long)
                 a_hi, a_lo = attn(qkv_hi, qkv_lo, qkv32)
                 _, _, h = ly["out"](a_hi, a_lo, P, residual=h, out_f32=True, out_planes=False)
                 y_hi, y_lo, _ = ops.layernorm(h, *ly["ln2"], cfg.enc_ln_eps)
@@ -361,12 +368,16 @@ class DiDiSampler:
             c_hi, c_lo, ctx = ops.layernorm(h, *e["ln_f"], cfg.enc_ln_eps, f32=True)
         elif cfg.enc_kind == "t5":
             inner = A * cfg.enc_dkv
-            bias = self._t5_position_bias(Cn)
+            bias = None if long else self._t5_position_bias(Cn)
+            buckets = self._t5_buckets(Cn) if long else None  # the long form reads the table itself: no [heads, C, C] in memory
 
             wide_t5 = cfg.enc_dkv > 64 or cfg.enc_dkv % 8 != 0  # t5-3b / t5-11b: d_kv = 128
 
             def attn_t5(qkv_hi, qkv_lo, qkv_f32=None):
                 v = lambda t, i: t.view(B, Cn, 3 * inner)[:, :, i * inner:(i + 1) * inner]  # noqa: E731
+                if long:
+                    o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32, scale=1.0, rel_bias=(e["rel"], buckets))
+                    return ops.split(o.view(B * Cn, inner))
                 if wide_t5:
                     o = ops.attention_train(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, causal=False, key_mask=mask32, scale=1.0,
                                             pos_bias=bias)
@@ -378,7 +389,7 @@ class DiDiSampler:
             h = ops.embed_gather(input_ids, e["tok"]).view(B * Cn, E)
             for ly in e["layers"]:
                 y_hi, y_lo, _ = ops.rmsnorm(h, ly["ln1"], cfg.enc_ln_eps)
-                qkv_hi, qkv_lo, qkv32 = ly["qkv"](y_hi, y_lo, P, out_f32=wide_t5)
+                qkv_hi, qkv_lo, qkv32 = ly["qkv"](y_hi, y_lo, P, out_f32=wide_t5 or long)
                 a_hi, a_lo = attn_t5(qkv_hi, qkv_lo, qkv32)
                 _, _, h = ly["out"](a_hi, a_lo, P, residual=h, out_f32=True, out_planes=False)
                 y_hi, y_lo, _ = ops.rmsnorm(h, ly["ln2"], cfg.enc_ln_eps)
@@ -398,7 +409,7 @@ class DiDiSampler:
                               tok_type0=e["tok0"], ln_gamma=e["eln"][0], ln_beta=e["eln"][1], ln_eps=1e-12, h_hi=h_hi, h_lo=h_lo)
             ctx = None
             for ly in e["layers"]:
-                qkv_hi, qkv_lo, qkv32 = ly["qkv"](h_hi, h_lo, P, out_f32=wide_heads)
+                qkv_hi, qkv_lo, qkv32 = ly["qkv"](h_hi, h_lo, P, out_f32=wide_heads or long)
                 a_hi, a_lo = attn(qkv_hi, qkv_lo, qkv32)
                 _, _, t = ly["out"](a_hi, a_lo, P, residual_planes=(h_hi, h_lo), out_f32=True, out_planes=False)
                 h_hi, h_lo, _ = ops.layernorm(t, *ly["ln1"], 1e-12)
@@ -408,18 +419,21 @@ class DiDiSampler:
             c_hi, c_lo = h_hi, h_lo
         return c_hi, c_lo, ctx
 
+    def _t5_buckets(self, c):
+        """Buckets of the distances that c positions have (the encoder's rule is computed once; farther distances share its ends)."""
+        e, cfg = self._enc, self.cfg
+        if "buckets" not in e:
+            e["buckets"] = ops.relative_buckets(cfg.enc_rel_buckets, cfg.enc_rel_max_distance, device=self.device)
+        far = e["buckets"].numel() // 2
+        m = min(far, max(1, c - 1))
+        return e["buckets"][far - m:far + m + 1].contiguous()
+
     def _t5_position_bias(self, c):
         """[heads, C, C] fp32 relative position bias of T5Attention.compute_bias (HF:models/t5/modeling_t5.py:217-279),
-        bidirectional buckets; index arithmetic on the host (C <= 96), one gather of the block-0 table on the device."""
-        e, cfg = self._enc, self.cfg
+        bidirectional buckets: one kernel from the block-0 table; the attention of up to ATTENTION_MAX_LEN positions reads it."""
+        e = self._enc
         if c not in e["bias_cache"]:
-            nb, max_exact = cfg.enc_rel_buckets // 2, cfg.enc_rel_buckets // 4
-            rel = torch.arange(c)[None, :] - torch.arange(c)[:, None]  # memory position - query position
-            rp = rel.abs()
-            large = max_exact + (torch.log(rp.float() / max_exact) / math.log(cfg.enc_rel_max_distance / max_exact) * (nb - max_exact)).to(torch.long)
-            large = torch.min(large, torch.full_like(large, nb - 1))
-            bucket = (rel > 0).long() * nb + torch.where(rp < max_exact, rp, large)
-            e["bias_cache"] = {c: e["rel"][bucket.to(self.device)].permute(2, 0, 1).contiguous()}
+            e["bias_cache"] = {c: ops.relative_bias(e["rel"], self._t5_buckets(c), c, c)}
         return e["bias_cache"][c]
 
     # ------------------------------------------------------------------ buffers + hoisted cross K/V

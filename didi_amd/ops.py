@@ -533,6 +533,9 @@ def _attn_train_args(q, k, v, heads, causal, key_mask, scale, drop_p, seed, offs
     return a
 
 
+ATTENTION_MAX_LEN = 96  # positions of ``attention`` / ``attention_train`` and their backward; past them: ``cross_attention``
+
+
 def attention_train(q, k, v, heads, causal=False, key_mask=None, scale=None, drop_p=0.0, seed=0, offset=0, pos_bias=None):
     """Training-step attention in fp32: O = dropout(softmax(q k^T scale + pos_bias + masks)) v -> fp32 [B, Sq, heads*D] contiguous.
     q/k/v fp32 [B, S, heads*D] (row-strided views of a fused projection are fine); ``pos_bias`` fp32 [heads, Sq, Sk] (T5)."""
@@ -713,7 +716,7 @@ def _rows(name, t, shape, dtype, device):
     return t.data_ptr(), batch if B > 1 else 0, row if S > 1 else W
 
 
-_PACK = struct.Struct("@9if2P3P3P3q3i2PqiP2P2if2QPqi3P3q3iPPN").pack  # didi_long_attn_args
+_PACK = struct.Struct("@9if2P3P3q3i2PqiP2P2if2QPqi3P3q3iPPN").pack  # didi_long_attn_args
 _NO_GRADS = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
@@ -756,7 +759,7 @@ def _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, s
         raise ValueError(f"drop_p={drop_p} must be in [0, 1)")
     if not drop_p:
         seed = offset = 0
-    before = (B, heads, kv_heads, Sq, Sk, D, code, 1 if causal else 0, q_start, scale, mask, count, Q, K, V, 0, 0, 0, qb, kb, vb, ldq, ldk, ldv)
+    before = (B, heads, kv_heads, Sq, Sk, D, code, 1 if causal else 0, q_start, scale, mask, count, Q, K, V, qb, kb, vb, ldq, ldk, ldv)
     return before, (table, buckets, nb, maxd, drop_p, seed, offset)
 
 

@@ -293,6 +293,21 @@ class DiDiTrainer:
 
         def drop(x, residual, off):  # hidden dropout (+ residual), or its backward with residual = None
             return ops.dropout_add(x, residual, ph, dseed, off)
+
+        long = max(S, Cn) > ops.ATTENTION_MAX_LEN
+
+        def attend(q, k, v, **kw):  # -> [M, H] and what the backward wants of the forward; one dropout mask stream in both forms
+            kw.update(drop_p=pa, seed=dseed)
+            o, stat = ops.cross_attention(q, k, v, A, need_grad=True, **kw) if long else (ops.attention_train(q, k, v, A, **kw), None)
+            return o.view(M, H), stat
+
+        def attend_backward(q, k, v, o, stat, do, out, **kw):
+            kw.update(drop_p=pa, seed=dseed, out=out)
+            if long:
+                ops.cross_attention_backward(q, k, v, o.view(B, S, H), stat, do.view(B, S, H), A, **kw)
+            else:
+                ops.attention_backward(q, k, v, do.view(B, S, H), A, **kw)
+
         # ---- noising (model.py:202-207)
         emb = ops.embed_gather(ids, P["emb.weight"])
         seed = 0
@@ -339,8 +354,7 @@ class DiDiTrainer:
             _, _, qkv = self._linear(L["qkv"], h_hi, h_lo, out_planes=False)
             q3 = qkv.view(B, S, 3 * H)
             s["off_sa"] = site()
-            att = ops.attention_train(q3[:, :, :H], q3[:, :, H:2 * H], q3[:, :, 2 * H:], A, causal=True, drop_p=pa, seed=dseed,
-                                      offset=s["off_sa"]).view(M, H)
+            att, s["stat_sa"] = attend(q3[:, :, :H], q3[:, :, H:2 * H], q3[:, :, 2 * H:], causal=True, offset=s["off_sa"])
             a_hi, a_lo = ops.split(att, dtype=pd)
             s["qkv"], s["att"], s["attp"] = qkv, att, (a_hi, a_lo)
             s["off_o"] = site()
@@ -355,8 +369,7 @@ class DiDiTrainer:
             _, _, ckv = self._linear(L["ckv"], x_hi, x_lo, out_planes=False)
             kv3 = ckv.view(B, Cn, 2 * H)
             s["off_ca"] = site()
-            catt = ops.attention_train(cq.view(B, S, H), kv3[:, :, :H], kv3[:, :, H:], A, causal=False, key_mask=mask32, drop_p=pa,
-                                       seed=dseed, offset=s["off_ca"]).view(M, H)
+            catt, s["stat_ca"] = attend(cq.view(B, S, H), kv3[:, :, :H], kv3[:, :, H:], key_mask=mask32, offset=s["off_ca"])
             ca_hi, ca_lo = ops.split(catt, dtype=pd)
             s["cq"], s["ckv"], s["catt"], s["cattp"] = cq, ckv, catt, (ca_hi, ca_lo)
             s["off_co"] = site()
@@ -448,8 +461,8 @@ class DiDiTrainer:
             ckv = s["ckv"].view(B, Cn, 2 * H)
             dckv = torch.empty_like(ckv)
             dcq = torch.empty((B, S, H), dtype=torch.float32, device=dev)
-            ops.attention_backward(s["cq"].view(B, S, H), ckv[:, :, :H], ckv[:, :, H:], dcatt.view(B, S, H), A, causal=False, key_mask=mask32,
-                                   out=(dcq, dckv[:, :, :H], dckv[:, :, H:]), drop_p=pa, seed=dseed, offset=s["off_ca"])
+            attend_backward(s["cq"].view(B, S, H), ckv[:, :, :H], ckv[:, :, H:], s["catt"], s["stat_ca"], dcatt, (dcq, dckv[:, :, :H], dckv[:, :, H:]),
+                            key_mask=mask32, offset=s["off_ca"])
             dh1, dW, dbias = self._linear_bwd(dcq.view(M, H), s["h1"], L["cq"], residual=ds2, A_planes=s["h1p"])
             put(ln["cq"], dW, dbias)
             dctx_l, dW, dbias = self._linear_bwd(dckv.view(B * Cn, 2 * H), ctx.view(B * Cn, H), L["ckv"], residual=dctx, need_dA=need_dctx, A_planes=(x_hi, x_lo))
@@ -463,8 +476,8 @@ class DiDiTrainer:
             put(ln["o"], dW, dbias)
             qkv = s["qkv"].view(B, S, 3 * H)
             dqkv = torch.empty_like(qkv)
-            ops.attention_backward(qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], datt.view(B, S, H), A, causal=True,
-                                   out=(dqkv[:, :, :H], dqkv[:, :, H:2 * H], dqkv[:, :, 2 * H:]), drop_p=pa, seed=dseed, offset=s["off_sa"])
+            attend_backward(qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], s["att"], s["stat_sa"], datt,
+                            (dqkv[:, :, :H], dqkv[:, :, H:2 * H], dqkv[:, :, 2 * H:]), causal=True, offset=s["off_sa"])
             dh0, dW, dbias = self._linear_bwd(dqkv.view(M, 3 * H), s["h0"], L["qkv"], residual=ds1, A_planes=s["h0p"])
             for j, key in enumerate(("q", "k", "v")):
                 put(ln[key], dW[j * H:(j + 1) * H].contiguous(), dbias[j * H:(j + 1) * H].contiguous())

@@ -25,7 +25,7 @@ def args(**kw):
     (BAD, dict(B=-1)), (BAD, dict(heads=3)), (BAD, dict(kv_heads=0)), (BAD, dict(Sq=-1)), (BAD, dict(D=0)), (BAD, dict(dtype=3)), (BAD, dict(q_start=-1)),
     (BAD, dict(scale=-1.0)), (BAD, dict(scale=float("nan"))), (BAD, dict(scale=float("inf"))), (BAD, dict(drop_p=1.0)), (BAD, dict(drop_p=-0.1)),
     (BAD, dict(Q=None)), (BAD, dict(K=None)), (BAD, dict(O=None)), (BAD, dict(Q=P + 2)), (BAD, dict(V=P + 8)), (BAD, dict(ldq=255)), (BAD, dict(ldk=132)),
-    (BAD, dict(ldk=64)), (BAD, dict(k_batch=2561)), (BAD, dict(k_batch=-128)), (BAD, dict(o_batch=2048)), (BAD, dict(Q_lo=P)), (BAD, dict(table=P)),
+    (BAD, dict(ldk=64)), (BAD, dict(k_batch=2561)), (BAD, dict(k_batch=-128)), (BAD, dict(o_batch=2048)), (BAD, dict(table=P)),
     (BAD, dict(table=P, buckets=P, num_buckets=0, max_distance=8)), (BAD, dict(dtable=P)), (BAD, dict(workspace=P + 4)),
     (UNSUPPORTED, dict(D=136)), (UNSUPPORTED, dict(D=60)), (UNSUPPORTED, dict(table=P, buckets=P, num_buckets=8, max_distance=513)),
     (UNSUPPORTED, dict(table=P, buckets=P, num_buckets=1025, max_distance=8)), (UNSUPPORTED, dict(Sk=(1 << 30) + 1)), (UNSUPPORTED, dict(q_start=1 << 30)),
@@ -38,7 +38,7 @@ def test_forward_refuses(rc, kw):
 
 
 @pytest.mark.parametrize("rc,kw", [(BAD, dict(dO=None)), (BAD, dict(dK=None)), (BAD, dict(lse=None)), (BAD, dict(dk_batch=0)), (BAD, dict(dv_batch=128)),
-                                   (BAD, dict(Q_lo=P, K_lo=P, V_lo=P)), (BAD, dict(lddq=8)), (WORKSPACE, dict(workspace_bytes=16)), (WORKSPACE, dict(workspace=None))])
+                                   (BAD, dict(lddq=8)), (WORKSPACE, dict(workspace_bytes=16)), (WORKSPACE, dict(workspace=None))])
 def test_backward_refuses(rc, kw):
     assert lib.didi_long_attention_backward(args(**kw), None) == rc
 
