@@ -76,6 +76,32 @@ __global__ void __launch_bounds__(256) la_bias_dense(const void* table, const in
     }
 }
 
+// first and last distance whose bucket differs from that of the end on its side; every thread gets both (sh: 8 ints)
+__device__ __forceinline__ void bias_range(const LaParams& p, int* sh, int tid, int& lo, int& hi) {
+    const int a = p.map[0], z = p.map[2 * p.maxd];
+    int l = p.maxd + 1, h = -p.maxd - 1;
+    for (int x = tid; x <= 2 * p.maxd; x += 256) {
+        const int t = p.map[x];
+        if (t != a) l = min(l, x - p.maxd);
+        if (t != z) h = max(h, x - p.maxd);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        l = min(l, __shfl_xor(l, o, 64));
+        h = max(h, __shfl_xor(h, o, 64));
+    }
+    if ((tid & 63) == 0) {
+        sh[tid >> 6] = l;
+        sh[4 + (tid >> 6)] = h;
+    }
+    __syncthreads();
+    lo = min(min(sh[0], sh[1]), min(sh[2], sh[3]));
+    hi = max(max(sh[4], sh[5]), max(sh[6], sh[7]));
+    // one bucket throughout (or two that meet): everything left of lo is the left end's, everything from lo on the right end's
+    hi = max(hi, lo - 1);
+    lo = min(lo, hi + 1);
+}
+
 // Sums of a dense gradient [B][H][Sq][Sk] by distance: a workgroup takes `rows` rows of one (dialog, head).  The distances at which the map
 // changes are summed along their diagonals, one thread each (neighbouring threads read neighbouring columns); what lies left and right of
 // them goes, 16 bytes at a time, into two sums.  Bound by the one read of the gradient.
@@ -383,7 +409,7 @@ extern "C" int didi_relative_bias_backward(const void* dbias, const int32_t* buc
 #undef DIDI_GRAD
         DIDI_LAUNCH_CHECK();
     }
-    const size_t lds = (size_t)5 * (2 * max_distance + 3) * 4;
+    const size_t lds = table_lds(max_distance, 1024);
 #define DIDI_SUM(T) la_table_sum<T><<<heads, 1024, lds, st>>>(p.tpart, buckets, any ? B : 0, heads, std::max(parts, 1), num_buckets, max_distance, dtable)
     if (dtype == DIDI_DT_FP32) DIDI_SUM(EF32);
     else if (dtype == DIDI_DT_FP16) DIDI_SUM(E16<true>);

@@ -56,6 +56,8 @@ struct LaParams {
     uint32_t images;  // bytes of LDS before the bias
     int ns, nrt, per;  // splits of the contraction, row (key) tiles, contraction tiles of a split
     float *part, *ml, *part2, *tpart;
+    void* dtable;  // la_backward_kv: written by the workgroups behind the keys', from tparts arrays per (dialog, head)
+    int tparts;
 };
 
 // ---- element types: how operands lie in memory, what multiplies them
@@ -114,6 +116,10 @@ struct Frag {
             x[c] = make_uint4(0, 0, 0, 0);
             if (ok && col < D) x[c] = T::load(p, off + col);
         }
+    }
+    __device__ void clear() {
+#pragma unroll
+        for (int c = 0; c < N; ++c) x[c] = make_uint4(0, 0, 0, 0);
     }
     // The loads have landed.  Said once before a loop that counts its copies: the compiler would otherwise wait for them -- and with them for
     // every copy on its way -- at their first use in each of its turns.
@@ -342,7 +348,8 @@ __device__ __forceinline__ int visible_end(const LaParams& p, int b) {
 }
 
 // Which keys of a dialog a workgroup's rows may see, 64 a word: the key mask is turned into bits ahead of the tiles, 64 words at a time into a
-// ring of 128 in LDS; without a mask the padding alone decides and nothing is kept.
+// ring of 128 in LDS; without a mask the padding alone decides and nothing is kept.  Where the first window holds more than four words a wave asks
+// for eight at once: one after the other their latencies were 2 us of a launch over 777 keys (127 keys: 25 us with the loop, 27 with the longer code).
 struct Keys {
     const int32_t* row;  // the dialog's key mask or null
     uint64_t* ring;
@@ -357,13 +364,29 @@ struct Keys {
         }
     }
     __device__ __forceinline__ void start(const LaParams& p, int b, int end_, uint64_t* ring_, int key0, int tid) {
-        row = p.mask ? p.mask + (int64_t)b * p.Sk : nullptr;
+        row = p.mask && end_ > 0 ? p.mask + (int64_t)b * p.Sk : nullptr;
         ring = ring_;
         end = end_;
         window = key0 >> 12;
         if (row) {
-            fill(window, tid);
-            fill(window + 1, tid);
+            if (end - (window << 12) <= 256) {
+                fill(window, tid);
+            } else {
+#pragma unroll 1
+                for (int w = window * 64; w < window * 64 + 64 && w * 64 < end; w += 32) {
+                    const int lane = tid & 63, w0 = w + (tid >> 6);
+                    int m[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) m[j] = row[min((w0 + 4 * j) * 64 + lane, end - 1)];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int word = w0 + 4 * j;
+                        const uint64_t bits = __ballot(word * 64 + lane < end && m[j] != 0);
+                        if (lane == 0 && word * 64 < end) ring[word & 127] = bits;
+                    }
+                }
+                fill(window + 1, tid);
+            }
             barrier();
         }
     }
@@ -387,44 +410,70 @@ struct Keys {
     }
 };
 
-// The bias as a function of the distance alone, for one head, in base-2 units: bv[d + maxd + PADB] for |d| <= maxd + PADB; outside
-// [lo, hi] the buckets are those of the ends.  A bucket outside the table gives NaN.
+// The bias as a function of the distance alone, for one head, in base-2 units: bv[d + maxd + PADB] for |d| <= maxd + PADB.  A bucket outside the
+// table gives NaN.  Bucket and value are two loads that wait for one another, so a kernel asks for the buckets first, for the values after its index
+// arithmetic, and stores them behind its other loads (512 distances at once; done in one place they took 2 us of a launch).
+template <class T>
 struct Bias {
-    float *v, left, right;
-    int lo, hi;
+    int t[2];
+    float f[2];
+    __device__ __forceinline__ void ask(const LaParams& p, int x0, int tid) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) t[k] = p.map[min(max(x0 + tid + 256 * k - PADB, 0), 2 * p.maxd)];
+    }
+    __device__ __forceinline__ void gather(const LaParams& p, int head) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) f[k] = T::elem(p.table, (int64_t)min(max(t[k], 0), p.nb - 1) * p.H + head);
+    }
+    __device__ __forceinline__ void store(const LaParams& p, float* v, int x0, int tid) const {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int x = x0 + tid + 256 * k;
+            if (x < 2 * p.maxd + 1 + 2 * PADB) v[x] = t[k] >= 0 && t[k] < p.nb ? f[k] * LOG2E : __builtin_nanf("");
+        }
+    }
+    // stores what was asked for and the rest; [lo, hi]: outside these distances the buckets are those of the ends (sh: 8 ints)
+    __device__ __forceinline__ void finish(const LaParams& p, int head, float* v, int* sh, int tid, int& lo, int& hi) {
+        const int a = p.map[0], z = p.map[2 * p.maxd];
+        int l = p.maxd + 1, h = -p.maxd - 1;
+        for (int x0 = 0; x0 < 2 * p.maxd + 1 + 2 * PADB; x0 += 512) {
+            if (x0 > 0) {
+                ask(p, x0, tid);
+                gather(p, head);
+            }
+            store(p, v, x0, tid);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int d = min(max(x0 + tid + 256 * k - PADB, 0), 2 * p.maxd) - p.maxd;
+                if (t[k] != a) l = min(l, d);
+                if (t[k] != z) h = max(h, d);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            l = min(l, __shfl_xor(l, o, 64));
+            h = max(h, __shfl_xor(h, o, 64));
+        }
+        if ((tid & 63) == 0) {
+            sh[tid >> 6] = l;
+            sh[4 + (tid >> 6)] = h;
+        }
+        barrier();
+        lo = min(min(sh[0], sh[1]), min(sh[2], sh[3]));
+        hi = max(max(sh[4], sh[5]), max(sh[6], sh[7]));
+        // one bucket throughout (or two that meet): everything left of lo is the left end's, everything from lo on the right end's
+        hi = max(hi, lo - 1);
+        lo = min(lo, hi + 1);
+    }
 };
 template <class T>
 __device__ __forceinline__ void bias_fill(const LaParams& p, int head, float* v, int tid) {
-    const int n = 2 * p.maxd + 1 + 2 * PADB;
-    for (int x = tid; x < n; x += 256) {
-        const int t = p.map[min(max(x - PADB, 0), 2 * p.maxd)];
-        v[x] = t >= 0 && t < p.nb ? T::elem(p.table, (int64_t)t * p.H + head) * LOG2E : __builtin_nanf("");
+    for (int x0 = 0; x0 < 2 * p.maxd + 1 + 2 * PADB; x0 += 512) {
+        Bias<T> b;
+        b.ask(p, x0, tid);
+        b.gather(p, head);
+        b.store(p, v, x0, tid);
     }
-}
-// first and last distance whose bucket differs from that of the end on its side; every thread gets both (sh: 8 ints)
-__device__ __forceinline__ void bias_range(const LaParams& p, int* sh, int tid, int& lo, int& hi) {
-    const int a = p.map[0], z = p.map[2 * p.maxd];
-    int l = p.maxd + 1, h = -p.maxd - 1;
-    for (int x = tid; x <= 2 * p.maxd; x += 256) {
-        const int t = p.map[x];
-        if (t != a) l = min(l, x - p.maxd);
-        if (t != z) h = max(h, x - p.maxd);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        l = min(l, __shfl_xor(l, o, 64));
-        h = max(h, __shfl_xor(h, o, 64));
-    }
-    if ((tid & 63) == 0) {
-        sh[tid >> 6] = l;
-        sh[4 + (tid >> 6)] = h;
-    }
-    __syncthreads();
-    lo = min(min(sh[0], sh[1]), min(sh[2], sh[3]));
-    hi = max(max(sh[4], sh[5]), max(sh[6], sh[7]));
-    // one bucket throughout (or two that meet): everything left of lo is the left end's, everything from lo on the right end's
-    hi = max(hi, lo - 1);
-    lo = min(lo, hi + 1);
 }
 
 // keep (1 / (1 - p)) or drop (0) of the 4 probabilities of keys j0 .. j0 + 3 (j0 % 4 == 0) of one row: the stream of
@@ -467,6 +516,8 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ uint64_t ring[128];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    Bias<T> bias;
+    if constexpr (BIAS) bias.ask(p, 0, tid);
     if constexpr (T::F16) f16_saturate_mode();
     const int rt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.HG), hg = (int)blockIdx.x - b * p.HG;
     const int head0 = p.Gr > 1 ? hg * p.Gr : hg, kvh = p.Gr > 1 ? hg : p.G > 1 ? hg / p.G : hg;
@@ -482,6 +533,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
 
     const int r = rw + (lane & 31), g = r < R ? row_group(p, r) : 0, i = r < R ? r - g * p.Sq : 0, head = head0 + g, pos = p.q_start + i;
     const int64_t rowid = ((int64_t)b * p.H + head) * p.Sq + i;
+    if constexpr (BIAS) bias.gather(p, head0);
     Frag<T, DP> q;
     q.load(p.Q, (int64_t)b * p.qb + (int64_t)i * p.ldq + head * p.D, r < R, p.D, h);
     const int64_t kbase = (int64_t)b * p.kb + kvh * p.D, vbase = (int64_t)b * p.vb + kvh * p.D;
@@ -505,10 +557,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
 
     float* bv = reinterpret_cast<float*>(smem + p.images);
     int blo = 0, bhi = -1;
-    if constexpr (BIAS) {
-        bias_fill<T>(p, head0, bv, tid);
-        bias_range(p, reinterpret_cast<int*>(bv + 2 * p.maxd + 1 + 2 * PADB), tid, blo, bhi);
-    }
+    if constexpr (BIAS) bias.finish(p, head0, bv, reinterpret_cast<int*>(bv + 2 * p.maxd + 1 + 2 * PADB), tid, blo, bhi);
 
     f32x16 o[DP / 32];
 #pragma unroll
@@ -759,6 +808,8 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ uint64_t ring[128];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    Bias<T> bias;
+    if constexpr (BIAS) bias.ask(p, 0, tid);
     if constexpr (T::F16) f16_saturate_mode();
     const int rt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.HG), hg = (int)blockIdx.x - b * p.HG;
     const int head0 = p.Gr > 1 ? hg * p.Gr : hg, kvh = p.Gr > 1 ? hg : p.G > 1 ? hg / p.G : hg;
@@ -775,6 +826,14 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     }
     const int tiles = (kend + C::BN - 1) / C::BN;
     const int t0 = split * p.per, t1 = min(tiles, t0 + p.per);
+
+    if constexpr (BIAS) bias.gather(p, head0);
+    const int64_t oo = (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D;
+    Frag<T, DP> q, go, o;
+    q.load(p.Q, (int64_t)b * p.qb + (int64_t)i * p.ldq + head * p.D, rok, p.D, h);
+    go.load(p.dO, (int64_t)b * p.dob + (int64_t)i * p.lddo + head * p.D, rok, p.D, h);
+    o.load(p.O[0], oo, rok, p.D, h);
+    const float lse = rok ? p.lse[rowid] : -INFINITY;
 
     const int64_t kbase = (int64_t)b * p.kb + kvh * p.D, vbase = (int64_t)b * p.vb + kvh * p.D;
     KV tk, tv;
@@ -793,14 +852,8 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     for (int k = 0; k < C::NS - 1; ++k)
         if (t0 + k < t1) issue(t0 + k);
 
-    Frag<T, DP> q, go;
-    q.load(p.Q, (int64_t)b * p.qb + (int64_t)i * p.ldq + head * p.D, rok, p.D, h);
-    go.load(p.dO, (int64_t)b * p.dob + (int64_t)i * p.lddo + head * p.D, rok, p.D, h);
     float delta = 0.f, norm = 0.f;
     {
-        const int64_t oo = (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D;
-        Frag<T, DP> o;
-        o.load(p.O[0], oo, rok, p.D, h);
 #pragma unroll
         for (int c = 0; c < Frag<T, DP>::N; ++c) {
             if constexpr (T::F32) {
@@ -833,7 +886,6 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     }
     norm = __builtin_amdgcn_sqrtf(norm);
     const float fs = T::F16 ? pow2_scale(norm) : 1.f;
-    const float lse = rok ? p.lse[rowid] : -INFINITY;
     const float sub = lse == -INFINITY ? -INFINITY : -lse * LOG2E;  // a row that sees nothing: p = exp2(-inf) = 0
     if (split == 0 && wk == 0 && rok && h == 0) {  // for la_backward_kv
         const int64_t rows_all = (int64_t)p.B * p.H * p.Sq;
@@ -842,15 +894,17 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
         if constexpr (T::F16) p.rows[2 * rows_all + rowid] = norm;
     }
 
-    float* bv = reinterpret_cast<float*>(smem + p.images);
+    float* bv = reinterpret_cast<float*>(smem + p.images) + 4 * 2048;  // behind the four waves' blocks of diagonals
     int blo = 0, bhi = -1;
     const int len = dist_len(p.maxd);
     float* acc_d = bv + len + 8;  // [4 waves][len]
-    float* skew = acc_d + 4 * len + wave * 2048;
+    float* skew = reinterpret_cast<float*>(smem + p.images) + wave * 2048;
     if constexpr (BIAS) {
-        bias_fill<T>(p, head0, bv, tid);
-        for (int x = tid; x < 4 * len + 4 * 2048; x += 256) acc_d[x] = 0.f;
-        bias_range(p, reinterpret_cast<int*>(bv + len), tid, blo, bhi);
+        if (p.tpart) {
+            for (int x = lane * 4; x < 2048; x += 256) *reinterpret_cast<float4*>(skew + x) = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int x = tid; x < 4 * len; x += 256) acc_d[x] = 0.f;
+        }
+        bias.finish(p, head0, bv, reinterpret_cast<int*>(bv + len), tid, blo, bhi);
     }
     float* mine_d = acc_d + wave * len;
     float far_l = 0.f, far_r = 0.f;
@@ -1025,28 +1079,37 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
 }
 
 // dtable[t][h] from the sums by distance of `parts` workgroups per (dialog, head) -- tpart [B][H][parts][2 maxd + 1 distances, left, right] --
-// added in a fixed order; one workgroup per head
-template <class T>
-__global__ void __launch_bounds__(1024) la_table_sum(const float* tpart, const int32_t* map, int B, int H, int parts, int nb, int maxd, void* out) {
-    extern __shared__ float dist[];  // [4][nd + 2], then the map
-    const int h = blockIdx.x, nd = 2 * maxd + 1, n = nd + 2, tid = threadIdx.x, grp = tid >> 8;
-    for (int x = tid; x < nd; x += 1024) reinterpret_cast<int*>(dist + 4 * n)[x] = map[x];
+// added in a fixed order by one workgroup of N threads per head.  Latency is all there is to it, so eight loads are in flight at a time, and the
+// attention's backward gives these workgroups a place in la_backward_kv's launch (a launch of their own took 7 us).
+constexpr int table_lds(int maxd, int threads) { return (threads / 256 + 1) * (2 * maxd + 3) * 4; }
+template <class T, int N>
+__device__ __forceinline__ void table_sum(const float* tpart, const int32_t* map, int B, int H, int parts, int nb, int maxd, void* out, int h, float* dist) {
+    constexpr int G = N / 256;
+    const int nd = 2 * maxd + 1, n = nd + 2, tid = threadIdx.x, grp = tid >> 8, total = B * parts;
+    int* bucket = reinterpret_cast<int*>(dist + G * n);  // dist: [G][n], then the map
+    for (int x = tid; x < nd; x += N) bucket[x] = map[x];
     for (int x = tid & 255; x < n; x += 256) {
         float sum = 0.f;
-        for (int b = 0; b < B; ++b) {
-            const float* at = tpart + ((int64_t)b * H + h) * parts * n + x;
-#pragma unroll 16
-            for (int k = grp; k < parts; k += 4) sum += at[(int64_t)k * n];
+        for (int e0 = grp; e0 < total; e0 += 8 * G) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int e = min(e0 + u * G, total - 1), b = e / parts;
+                v[u] = tpart[(((int64_t)b * H + h) * parts + (e - b * parts)) * n + x];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) sum += e0 + u * G < total ? v[u] : 0.f;
         }
         dist[grp * n + x] = sum;
     }
     __syncthreads();
-    for (int x = tid; x < n; x += 1024) dist[x] = (dist[x] + dist[n + x]) + (dist[2 * n + x] + dist[3 * n + x]);
-    __syncthreads();
+    if constexpr (G == 4) {
+        for (int x = tid; x < n; x += N) dist[x] = (dist[x] + dist[n + x]) + (dist[2 * n + x] + dist[3 * n + x]);
+        __syncthreads();
+    }
     // one wave per bucket: its lanes take the distances in turn
     const int lane = tid & 63;
-    const int* bucket = reinterpret_cast<const int*>(dist + 4 * n);
-    for (int t = tid >> 6; t < nb; t += 16) {
+    for (int t = tid >> 6; t < nb; t += N / 64) {
         float sum = 0.f;
 #pragma unroll 4
         for (int x = lane; x < nd; x += 64) sum += bucket[x] == t ? dist[x] : 0.f;
@@ -1058,6 +1121,11 @@ __global__ void __launch_bounds__(1024) la_table_sum(const float* tpart, const i
             else static_cast<u16*>(out)[(int64_t)t * H + h] = T::F16 ? f16_bits(sum) : bf16_bits(sum);
         }
     }
+}
+template <class T>
+__global__ void __launch_bounds__(1024) la_table_sum(const float* tpart, const int32_t* map, int B, int H, int parts, int nb, int maxd, void* out) {
+    extern __shared__ float dist[];
+    table_sum<T, 1024>(tpart, map, B, H, parts, nb, maxd, out, blockIdx.x, dist);
 }
 
 // out row = sum of the splits' partial rows
@@ -1104,17 +1172,28 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float top4[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    if constexpr (BIAS) {
+        if ((int)blockIdx.x >= p.B * p.Hk) {
+            if (blockIdx.y == 0 && blockIdx.z == 0)
+                table_sum<T, 256>(p.tpart, p.map, p.B, p.H, p.tparts, p.nb, p.maxd, p.dtable, (int)blockIdx.x - p.B * p.Hk, reinterpret_cast<float*>(smem));
+            return;
+        }
+    }
+    Bias<T> bias;
+    if constexpr (BIAS) bias.ask(p, 0, tid);
     if constexpr (T::F16) f16_saturate_mode();
     const int kt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.Hk), kvh = (int)blockIdx.x - b * p.Hk;
     const int kbase = kt * C::KEYS, wq = wave % WQ, kw = kbase + wave / WQ * 32, key = kw + (lane & 31);
     const int kend = visible_end(p, b);
-    const bool vis = key < kend && (!p.mask || p.mask[(int64_t)b * p.Sk + key] != 0);
+    const int seen = key < kend ? p.mask ? p.mask[(int64_t)b * p.Sk + key] : 1 : 0;
     const int64_t kvrow = (int64_t)b * p.kb + (int64_t)key * p.ldk + kvh * p.D, vrow = (int64_t)b * p.vb + (int64_t)key * p.ldv + kvh * p.D;
     const int64_t rows_all = (int64_t)p.B * p.H * p.Sq;
 
     const int qt0 = p.causal ? min(max(0, kbase - p.q_start), p.Sq) / C::BQ : 0, nq = (p.Sq + C::BQ - 1) / C::BQ - qt0;
     const int tiles = kbase < kend ? p.G * max(nq, 0) : 0;
     const int t0 = split * p.per, t1 = min(tiles, t0 + p.per);
+    int gcur = t0 < t1 ? t0 / nq : 0;
+    if constexpr (BIAS) bias.gather(p, kvh * p.G + gcur);
     QT tq, tg;
     tq.init(p.ldq, p.D, tid);
     tg.init(p.lddo, p.D, tid);
@@ -1134,8 +1213,8 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         if (t0 + k < t1) issue(t0 + k);
 
     Frag<T, DP> kf, vf;
-    kf.load(p.K, kvrow, vis, p.D, h);
-    vf.load(p.V, vrow, vis, p.D, h);
+    kf.load(p.K, kvrow, key < kend, p.D, h);
+    vf.load(p.V, vrow, key < kend, p.D, h);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
@@ -1145,12 +1224,15 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     float* bv = reinterpret_cast<float*>(smem + p.images);
     const int len = dist_len(p.maxd);
     int blo = 0, bhi = -1;
-    if constexpr (BIAS) bias_range(p, reinterpret_cast<int*>(bv + len), tid, blo, bhi);
+    if constexpr (BIAS) bias.finish(p, kvh * p.G + gcur, bv, reinterpret_cast<int*>(bv + len), tid, blo, bhi);
     float fs = 1.f;
     if constexpr (T::F16) {
         float top = 0.f;
         const float* norms = p.rows + 2 * rows_all + ((int64_t)b * p.H + kvh * p.G) * p.Sq;
-        for (int x = tid; x < p.G * p.Sq; x += 256) top = fmaxf(top, norms[x]);
+        const int n = p.G * p.Sq;
+        for (int x = tid; x < n; x += 1024)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, norms[min(x + 256 * k, n - 1)]);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         if (lane == 0) top4[wave] = top;
@@ -1158,9 +1240,13 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         fs = pow2_scale(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
     }
 
+    const bool vis = seen != 0;
+    if (!vis) {  // whatever a masked key holds, it is not multiplied
+        kf.clear();
+        vf.clear();
+    }
     kf.settle();
     vf.settle();
-    int gcur = -1;
     for (int t = t0; t < t1; ++t) {
         const int g = t / nq, i0 = (qt0 + t % nq) * C::BQ, head = kvh * p.G + g, qrow = wq * 32 * C::NT;
         if (C::NS > 3 && t + 2 < t1) wait_copies<(C::NS > 3 ? 2 : 0) * (2 * QT::NC + 2)>();
@@ -1432,11 +1518,11 @@ template <class T, int DP, int WQ>
 int launch_backward_kv(LaParams p, hipStream_t st) {
     static_assert(BwdKCfg<T, DP, WQ>::LDS + 8 * 1024 <= MAX_LDS, "the widest bias fits beside it");
     p.images = used_lds<BwdKCfg<T, DP, WQ>>(p);
-    const size_t lds = p.images + bias_lds(p);
+    const size_t lds = std::max<size_t>(p.images + bias_lds(p), p.dtable ? table_lds(p.maxd, 256) : 0);
     auto* fn = p.table ? &la_backward_kv<T, DP, WQ, true> : &la_backward_kv<T, DP, WQ, false>;
     static std::atomic<uint64_t> done[2];
     if (!lds_opt_in(fn, lds, done[p.table != nullptr])) return DIDI_ERR_LAUNCH;
-    fn<<<dim3(p.B * p.Hk, p.nrt, p.ns), 256, lds, st>>>(p);
+    fn<<<dim3(p.B * p.Hk + (p.dtable ? p.H : 0), p.nrt, p.ns), 256, lds, st>>>(p);
     DIDI_LAUNCH_CHECK();
     return DIDI_OK;
 }
@@ -1453,12 +1539,14 @@ int run_backward(LaParams p, const Plan& z, void* dtable, hipStream_t st) {
             DIDI_LAUNCH_CHECK();
         }
     }
-    if (dtable) {
-        la_table_sum<T><<<p.H, 1024, (size_t)5 * (2 * p.maxd + 3) * 4, st>>>(p.tpart, p.map, rows > 0 ? p.B : 0, p.H, z.q.nrt * z.q.ns, p.nb, p.maxd, dtable);
+    if (dtable && (krows == 0 || rows == 0)) {  // nothing to sum, or no launch to do it in
+        la_table_sum<T><<<p.H, 1024, table_lds(p.maxd, 1024), st>>>(p.tpart, p.map, rows > 0 ? p.B : 0, p.H, z.q.nrt * z.q.ns, p.nb, p.maxd, dtable);
         DIDI_LAUNCH_CHECK();
     }
     if (krows > 0) {
         set_cut(p, z.k);
+        p.dtable = rows > 0 ? dtable : nullptr;
+        p.tparts = z.q.nrt * z.q.ns;
         p.part2 = p.part + (int64_t)p.ns * krows * p.D;
         if (const int rc = z.k.wk == 1 ? launch_backward_kv<T, DP, 1>(p, st) : z.k.wk == 2 ? launch_backward_kv<T, DP, 2>(p, st) : launch_backward_kv<T, DP, max_share(T::F32, DP)>(p, st))
             return rc;
