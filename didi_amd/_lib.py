@@ -241,7 +241,7 @@ SYMBOLS = [
     ("didi_long_attention_forward", C.c_int, [C.POINTER(LongAttnArgs), C.c_void_p]),
     ("didi_long_attention_backward", C.c_int, [C.POINTER(LongAttnArgs), C.c_void_p]),
     ("didi_relative_bias", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
-    ("didi_relative_bias_backward_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    ("didi_relative_bias_backward_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     ("didi_relative_bias_backward", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                               C.c_void_p, C.c_void_p]),
     ("didi_event_create", C.c_int, [C.POINTER(C.c_void_p)]),

@@ -1067,7 +1067,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
         }
         __syncthreads();
         const int nd = 2 * p.maxd + 1;
-        float* out = p.tpart + (((int64_t)blockIdx.x * gridDim.y + rt) * gridDim.z + split) * (nd + 2);
+        float* out = p.tpart + ((((int64_t)hg * p.B + b) * gridDim.y + rt) * gridDim.z + split) * (nd + 2);
         for (int x = tid; x < nd; x += 256) out[x] = acc_d[PADB + x];
         if (wave < 2) {
             float sum = 0.f;
@@ -1078,8 +1078,8 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     }
 }
 
-// dtable[t][h] from the sums by distance of `parts` workgroups per (dialog, head) -- tpart [B][H][parts][2 maxd + 1 distances, left, right] --
-// added in a fixed order by one workgroup of N threads per head.  Latency is all there is to it, so eight loads are in flight at a time, and the
+// dtable[t][h] from the sums by distance of `parts` workgroups per (dialog, head) -- tpart [H][B][parts][2 maxd + 1 distances, left, right] --
+// added in a fixed order by one workgroup of N threads per head.  Latency is all there is to it, so sixteen loads are in flight at a time, and the
 // attention's backward gives these workgroups a place in la_backward_kv's launch (a launch of their own took 7 us).
 constexpr int table_lds(int maxd, int threads) { return (threads / 256 + 1) * (2 * maxd + 3) * 4; }
 template <class T, int N>
@@ -1090,15 +1090,14 @@ __device__ __forceinline__ void table_sum(const float* tpart, const int32_t* map
     for (int x = tid; x < nd; x += N) bucket[x] = map[x];
     for (int x = tid & 255; x < n; x += 256) {
         float sum = 0.f;
-        for (int e0 = grp; e0 < total; e0 += 8 * G) {
-            float v[8];
+        for (int e0 = grp; e0 < total; e0 += 16 * G) {
+            float v[16];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int e = min(e0 + u * G, total - 1), b = e / parts;
-                v[u] = tpart[(((int64_t)b * H + h) * parts + (e - b * parts)) * n + x];
+            for (int u = 0; u < 16; ++u) {
+                v[u] = tpart[((int64_t)h * total + min(e0 + u * G, total - 1)) * n + x];
             }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) sum += e0 + u * G < total ? v[u] : 0.f;
+            for (int u = 0; u < 16; ++u) sum += e0 + u * G < total ? v[u] : 0.f;
         }
         dist[grp * n + x] = sum;
     }

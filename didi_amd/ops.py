@@ -699,9 +699,10 @@ def relative_bias_backward(dbias, buckets, num_buckets, q_start=0):
         raise ValueError("dbias must be on the GPU")
     B, heads, Sq, Sk = (1, *dbias.shape) if dbias.dim() == 3 else dbias.shape
     dtable = torch.empty((num_buckets, heads), dtype=dbias.dtype, device=dev)
-    ws = torch.empty(lib.didi_relative_bias_backward_bytes(B, heads, maxd, Sq), dtype=torch.uint8, device=dev)
+    nbytes = lib.didi_relative_bias_backward_bytes(B, heads, maxd, Sq, Sk)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.check(_launch(dev, lib.didi_relative_bias_backward, dbias.data_ptr(), buckets.data_ptr(), dt, B, heads, num_buckets, maxd, Sq, Sk, q_start,
-                       dtable.data_ptr(), ws.data_ptr()), "relative_bias_backward")
+                       dtable.data_ptr(), ws.data_ptr() if nbytes else 0), "relative_bias_backward")
     return dtable
 
 

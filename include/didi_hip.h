@@ -741,7 +741,7 @@ int didi_long_attention_backward(const didi_long_attn_args* a, void* stream);
  * and the table's gradient from a dense one [B, heads, Sq, Sk] (summed over the B dialogs the bias was shared by).  dtype: all operands. */
 int didi_relative_bias(const void* table, const int32_t* buckets, int dtype, int heads, int num_buckets, int max_distance, int Sq, int Sk, int q_start,
                        void* out, void* stream);
-size_t didi_relative_bias_backward_bytes(int B, int heads, int max_distance, int Sq);
+size_t didi_relative_bias_backward_bytes(int B, int heads, int max_distance, int Sq, int Sk);
 int didi_relative_bias_backward(const void* dbias, const int32_t* buckets, int dtype, int B, int heads, int num_buckets, int max_distance, int Sq, int Sk,
                                 int q_start, void* dtable, void* workspace, void* stream);
 

@@ -280,7 +280,7 @@ def test_bucket_rule_matches_the_encoder(ops):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("B,H,Sq,Sk,q_start,bidirectional", [(1, 12, 64, 64, 0, True), (1, 1, 1, 1, 0, True), (2, 3, 77, 301, 0, False), (1, 2, 1, 1000, 999, False),
-                                                             (3, 2, 500, 33, 7, True), (1, 5, 130, 7, 0, True), (1, 2, 300, 1023, 723, True)])
+                                                             (3, 2, 500, 33, 7, True), (1, 5, 130, 7, 0, True), (1, 3, 64, 448, 7, True), (1, 3, 65, 64, 0, False), (1, 4, 400, 5, 3, False), (1, 2, 300, 1023, 723, True)])
 def test_dense_bias_and_its_gradient(ops, dtype, B, H, Sq, Sk, q_start, bidirectional):
     g = torch.Generator().manual_seed(Sq)
     table = torch.randn(32, H, generator=g).to(DT[dtype]).cuda()
