@@ -339,8 +339,10 @@ class DiDiSampler:
         if cfg.enc_kind != "t5" and Cn > e["pos"].shape[0]:
             raise ValueError(f"a context of {Cn} tokens: the encoder has {e['pos'].shape[0]} positions")
 
-        long = Cn > ops.ATTENTION_MAX_LEN  # past the lengths the attention kernels of a dialog are built for: fp32 attention of any length
-        wide_heads = E // A > 64 or (E // A) % 8 != 0  # e.g. Blenderbot-3B's 80-wide heads (configs/train.yaml:3)
+        D = cfg.enc_dkv if cfg.enc_kind == "t5" else E // A
+        wide_heads = D > 64 or D % 8 != 0  # e.g. Blenderbot-3B's 80-wide heads (configs/train.yaml:3), t5-3b / t5-11b: d_kv = 128
+        # past the sizes the attention kernels of a dialog are built for: fp32 attention of any length
+        long = Cn > ops.ATTENTION_MAX_LEN or (wide_heads and not ops.attention_train_fits(Cn, Cn, D))
 
         def attn(qkv_hi, qkv_lo, qkv_f32=None):
             v = lambda t, i: None if t is None else t.view(B, Cn, 3 * E)[:, :, i * E:(i + 1) * E]  # noqa: E731
@@ -371,14 +373,12 @@ class DiDiSampler:
             bias = None if long else self._t5_position_bias(Cn)
             buckets = self._t5_buckets(Cn) if long else None  # the long form reads the table itself: no [heads, C, C] in memory
 
-            wide_t5 = cfg.enc_dkv > 64 or cfg.enc_dkv % 8 != 0  # t5-3b / t5-11b: d_kv = 128
-
             def attn_t5(qkv_hi, qkv_lo, qkv_f32=None):
                 v = lambda t, i: t.view(B, Cn, 3 * inner)[:, :, i * inner:(i + 1) * inner]  # noqa: E731
                 if long:
                     o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32, scale=1.0, rel_bias=(e["rel"], buckets))
                     return ops.split(o.view(B * Cn, inner))
-                if wide_t5:
+                if wide_heads:
                     o = ops.attention_train(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, causal=False, key_mask=mask32, scale=1.0,
                                             pos_bias=bias)
                     return ops.split(o.view(B * Cn, inner))
@@ -389,7 +389,7 @@ class DiDiSampler:
             h = ops.embed_gather(input_ids, e["tok"]).view(B * Cn, E)
             for ly in e["layers"]:
                 y_hi, y_lo, _ = ops.rmsnorm(h, ly["ln1"], cfg.enc_ln_eps)
-                qkv_hi, qkv_lo, qkv32 = ly["qkv"](y_hi, y_lo, P, out_f32=wide_t5 or long)
+                qkv_hi, qkv_lo, qkv32 = ly["qkv"](y_hi, y_lo, P, out_f32=wide_heads or long)
                 a_hi, a_lo = attn_t5(qkv_hi, qkv_lo, qkv32)
                 _, _, h = ly["out"](a_hi, a_lo, P, residual=h, out_f32=True, out_planes=False)
                 y_hi, y_lo, _ = ops.rmsnorm(h, ly["ln2"], cfg.enc_ln_eps)

@@ -536,6 +536,11 @@ def _attn_train_args(q, k, v, heads, causal, key_mask, scale, drop_p, seed, offs
 ATTENTION_MAX_LEN = 96  # positions of ``attention`` / ``attention_train`` and their backward; past them: ``cross_attention``
 
 
+def attention_train_fits(Sq, Sk, D):
+    """Whether ``attention_train`` takes these sizes: one head's fp32 operands and scores share a workgroup's LDS."""
+    return max(Sq, Sk) <= ATTENTION_MAX_LEN and D <= 128 and 4 * ((Sq + 2 * Sk) * (D + 4) + Sq * ((Sk + 3) // 4 * 4 + 4)) <= 160 * 1024 - 256
+
+
 def attention_train(q, k, v, heads, causal=False, key_mask=None, scale=None, drop_p=0.0, seed=0, offset=0, pos_bias=None):
     """Training-step attention in fp32: O = dropout(softmax(q k^T scale + pos_bias + masks)) v -> fp32 [B, Sq, heads*D] contiguous.
     q/k/v fp32 [B, S, heads*D] (row-strided views of a fused projection are fine); ``pos_bias`` fp32 [heads, Sq, Sk] (T5)."""
