@@ -87,7 +87,7 @@ def reference(q, k, v, do, H, Hk, dtype, scale=None, causal=False, q_start=0, ke
     delta = (dO * o).sum(-1, keepdim=True)
     ds = p * (dp - delta)
     dpm = (dO.abs() @ V.abs().transpose(-1, -2)) * drop
-    lo = u * u if rel_bias is not None else u  # the remainder plane
+    lo = u if dtype == "fp32" else u * u  # 16 bits: with the remainder plane
     dd = (dO.abs() * o.abs()).sum(-1, keepdim=True) * (lo + n24(D)) + (dO.abs() * (A * (up + 2 * e + n24(Sk)))).sum(-1, keepdim=True)
     err = p * dd + ds.abs() * (2 * e + 2.0 ** -21) + p * dpm * n24(D)
     # fp16 score gradients are scaled by powers of two before their rounding: no subnormals in range; saturation-free
@@ -264,6 +264,21 @@ def test_gradients_against_differences(ops):
         # third-order rest of a five-point rule, fp32 outputs: |w|_1 2^-22 / h
         num = (8 * (at(1) - at(-1)) - (at(2) - at(-2))) / (12 * h)
         assert abs(num - float((g.double() * d.double()).sum())) < float(w.abs().sum()) * 2.0 ** -22 / h * 2, n
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D,causal", [(4, 16, 4, 495, 29, 80, False), (53, 12, 12, 19, 329, 32, True), (13, 6, 6, 31, 31, 64, True), (4, 8, 8, 57, 5, 40, False),
+                                                   (16, 32, 16, 470, 380, 16, False)])
+def test_query_and_key_gradients_lose_two_roundings(ops, dtype, B, H, Hk, Sq, Sk, D, causal):
+    """The score gradients are rounded once and so are the results, independently and alike: sqrt(2) of the error that rounding the exact
+    gradients makes, 1.5 with room for D = do . o."""
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=Sk)
+    got, _ = run(ops, q, k, v, do, H, Hk, causal=causal)
+    val, _ = reference(q, k, v, do, H, Hk, dtype, causal=causal)
+    for name in ("dq", "dk"):
+        want = val[name]
+        once = (want.to(DT[dtype]).double() - want).norm()
+        assert float((got[name].double() - want).norm() / once) <= 1.5, name
 
 
 def test_bucket_rule_matches_the_encoder(ops):
