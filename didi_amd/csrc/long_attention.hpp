@@ -497,6 +497,10 @@ constexpr int max_share(bool f32, int DP) { return f32 && DP > 64 ? 2 : 4; }
 // ------------------------------------------------------------------ forward
 // A workgroup's four waves are 4 / WK groups of 32 rows times WK parts of every key tile.  WK = 1: 128 rows share each key tile; WK = 2, 4:
 // fewer rows, the waves' shares are joined through LDS at the end (small batches, one token per dialog).
+// What bounds it: one token per dialog, the reading of keys and values -- 32 dialogs x 12 heads to 4096 keys, fp16: 48 us, 4.3 TB/s; 4 x 32 heads
+// over 8 of 128, 33001 keys, bf16: 100 us and 5 to join the splits, 5.1 TB/s.  Many rows, the products with the softmax between them (a wave's
+// products wait for its exponentials; other waves fill in): 2 x 16 heads of 128, 2048 x 8192, bf16: 310 us, 740 TFLOP/s.  Between them latency: a
+// launch over 500 keys is a prologue of 4 us and eight tiles that come one behind the other (64 x 12 heads, 63 x 512, fp16: 19 us).
 template <class T, int DP, int WK>
 struct FwdCfg {
     static constexpr int BN = tile_rows(T::F32, WK), NT = BN / (32 * WK);  // 32-key blocks a wave takes of a tile
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     }
 }
 
-// Joins the splits of the forward.  A workgroup takes 256 / (32 SL) rows: 32 lanes of four head-dim elements each, SL of them take the splits
+// Joins the splits of the forward: 5 us behind the longest (latency: it reads a few MB).  A workgroup takes 256 / (32 SL) rows: 32 lanes of four head-dim elements each, SL of them take the splits
 // in turn and are added in LDS (few rows, many splits: one token over a long context would otherwise wait for one split after the other).
 template <class T, int SL>
 __global__ void __launch_bounds__(256) la_join(LaParams p) {
@@ -786,6 +790,8 @@ __device__ __forceinline__ float pow2_scale(float norm) {
     return __builtin_bit_cast(float, (uint32_t)(127 + min(max(5 - e, -100), 100)) << 23);
 }
 
+// Bound by the products: 2 x 16 heads of 128, 2048 x 8192, bf16: 375 us for its three, 916 TFLOP/s.  Short ones by latency: causal fp32 128 x 128,
+// 96 heads of 64: 21 us, a third of it before the first tile (rows, bias, the sums' zeros), the rest two tiles of 6000 cycles.
 template <class T, int DP, int WK, bool BIAS>
 struct BwdQCfg {
     static constexpr int BN = tile_rows(T::F32, WK), NT = BN / (32 * WK);
@@ -1153,7 +1159,9 @@ __global__ void __launch_bounds__(256) la_sum_parts(const float* part, int ns, i
 
 // ------------------------------------------------------------------ backward: dK, dV
 // A workgroup owns 128 keys of one key head, its waves 32 each (lane = key: K and V rows live in registers); it walks tiles of BQ rows of
-// Q and dO of every head of the group.
+// Q and dO of every head of the group.  Bound by its four products and what they wait for: head dims past 64 (16 bits) hold dK, dV, K and V of a wave's
+// keys in 400 registers, so one wave a SIMD is all there is to hide an LDS read behind: 2 x 16 heads of 128, 2048 x 8192, bf16: 740 us, 619
+// TFLOP/s.  One launch for dK and one for dV have two waves a SIMD, but five products: 800 us.
 template <class T, int DP, int WQ>
 struct BwdKCfg {
     static constexpr int BQ = tile_rows(T::F32, WQ), NT = BQ / (32 * WQ);  // 32-row blocks a wave takes of a tile

@@ -4,7 +4,8 @@ Reference: src/diffusion/model.py:200-243 (training_step), :136-158 (AdamW(lr=1)
 configs/train.yaml:33-45 (optimizer block, gradient_clip_val), src/training.py:37 (DDP: gradient all-reduce, mean).
 The backward is written out by hand (no autograd): every piece is a libdidi_hip kernel --
   * Linear: dgrad and wgrad are MFMA GEMMs on transposed split planes, the bias gradient a column sum (ops.linear_backward);
-  * LayerNorm, GELU, tanh, softmax cross-entropy, embedding scatter-add, attention (probabilities recomputed): train.hip;
+  * LayerNorm, GELU, tanh, softmax cross-entropy, embedding scatter-add, attention (probabilities recomputed): train.hip; past 96
+    target or context tokens the attention of any length (long_attention.hip, fp32);
 torch owns the memory and does the B-element scalar arithmetic (per-dialog means, the clipping coefficient).
 What is trained: everything but the frozen context encoder (model.py:114-115): emb, time_embeds, classifier (or tied), adapter,
 the decoder.  ``decoder.embeddings.word_embeddings`` and ``decoder.pooler`` never receive a gradient in the reference (inputs

@@ -323,6 +323,18 @@ def test_a_bucket_outside_the_table_is_nan_and_collects_nothing(ops):
     assert float(got.sum()) == 2 * (400 - 17 - 18)
 
 
+def test_results_over_operands_are_refused(ops):
+    q, k, v, do = make(1, 2, 2, 8, 8, 32, "bf16")
+    with pytest.raises(ValueError):
+        ops.cross_attention(q, k, v, 2, out=q)
+    o, saved = ops.cross_attention(q, k, v, 2, need_grad=True)
+    fresh = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    for x in (q, k, v, o, do):
+        for n in range(3):
+            with pytest.raises(ValueError):
+                ops.cross_attention_backward(q, k, v, o, saved, do, 2, out=fresh[:n] + (x,) + fresh[n + 1:])
+
+
 def test_lengths_of_zero(ops):
     q, k, v, do = make(2, 2, 2, 5, 9, 32, "bf16")
     none = torch.zeros(2, 0, 64, dtype=torch.bfloat16, device="cuda")
