@@ -927,8 +927,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     q.settle();
     go.settle();
     for (int t = t0; t < t1; ++t) {
-        if (C::NS > 3 && t + 2 < t1) wait_copies<(C::NS > 3 ? 2 : 0) * 2 * KV::NC>();
-        else if (C::NS > 2 && t + 1 < t1) wait_copies<(C::NS > 2 ? 1 : 0) * 2 * KV::NC>();
+        if (C::NS > 2 && t + 1 < t1) wait_copies<(C::NS > 2 ? 1 : 0) * 2 * KV::NC>();
         else wait_copies<0>();
         barrier();
         keys.advance(t * C::BN, tid);
@@ -1259,8 +1258,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     vf.settle();
     for (int t = t0; t < t1; ++t) {
         const int g = t / nq, i0 = (qt0 + t % nq) * C::BQ, head = kvh * p.G + g, qrow = wq * 32 * C::NT;
-        if (C::NS > 3 && t + 2 < t1) wait_copies<(C::NS > 3 ? 2 : 0) * (2 * QT::NC + 2)>();
-        else if (C::NS > 2 && t + 1 < t1) wait_copies<(C::NS > 2 ? 1 : 0) * (2 * QT::NC + 2)>();
+        if (C::NS > 2 && t + 1 < t1) wait_copies<(C::NS > 2 ? 1 : 0) * (2 * QT::NC + 2)>();
         else wait_copies<0>();
         barrier();
         if (BIAS && g != gcur) {  // another head of the group: its bias

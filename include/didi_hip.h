@@ -368,7 +368,7 @@ int didi_mul_split(const float* a, const float* b, size_t n, uint16_t* y_hi, uin
  *                 behaviour), never NaN.
  * Q/K/V/O are split planes addressed as plane[(b*S + s) * ld + head*D + d]; lo planes may be NULL
  * together with precision DIDI_PREC_BF16.  D % 8 == 0, D <= 64; Sq, Sk <= 96 (dialogs are <= 84 tokens,
- * README.md:48-49 of the reference); ld % 8 == 0. */
+ * README.md:48-49 of the reference; longer: didi_long_attention_forward); ld % 8 == 0. */
 typedef struct didi_attn_args {
     int B, heads, Sq, Sk, D;
     int precision;
