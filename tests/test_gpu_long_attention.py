@@ -142,6 +142,8 @@ CASES = [
     (4, 6, 6, 256, 512, 64, "count", False, 0, True),
     (1, 1, 1, 40, 2000, 128, "mask", False, 0, False),
     (5, 8, 2, 2, 65, 8, "mask", False, 0, False),
+    (3, 2, 1, 2, 12501, 64, "mask", False, 0, False),  # more keys than the ring of mask words holds, split and
+    (1, 2, 2, 130, 9003, 32, "mask", True, 8873, False),  # in one piece
 ]
 
 
@@ -179,6 +181,18 @@ def test_forward_and_backward(ops, case, dtype):
     # rows without a key: exact zeros
     gone = ~fin.transpose(1, 2)  # [B, Sq, H]
     assert (got["o"].reshape(B, Sq, H, D)[gone] == 0).all() and (got["dq"].reshape(B, Sq, H, D)[gone] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", [(2, 2, 2, 70, 1300, 128), (1, 4, 2, 1200, 65, 64), (2, 2, 1, 33, 40, 96)])
+def test_the_widest_bias(ops, dtype, B, H, Hk, Sq, Sk, D):
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=Sq, scale_q=D ** -0.5)
+    buckets = (torch.arange(1025, dtype=torch.int32) * 7 % 1024).cuda()  # every distance another bucket, but for the ends'
+    table = (torch.randn(1024, H, generator=torch.Generator().manual_seed(5)) * 0.7).to(DT[dtype]).cuda()
+    kw = dict(masks("count", B, Sk), scale=1.0, rel_bias=(table, buckets))
+    got, _ = run(ops, q, k, v, do, H, Hk, **kw)
+    val, tol = reference(q, k, v, do, H, Hk, dtype, **kw)
+    compare(got, val, tol)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
