@@ -27,9 +27,10 @@ __global__ void __launch_bounds__(256) la_bias_dense(const void* table, const in
     int64_t c = (int64_t)blockIdx.x * chunks_per_wg + tid;
     const int64_t cend = min(chunks, ((int64_t)blockIdx.x + 1) * chunks_per_wg);
     if (c >= cend) return;
-    // row and column of the chunk's first element (the head's first chunk may begin before it: f < 0), then stepped by 256 chunks
+    // row and column of the chunk's first element, then stepped by 256 chunks.  The head's first chunk may begin before it: its row is then
+    // negative and its column the one that the steps go on from (0 <= j < Sk always)
     int64_t f = c * EPC - skew;
-    int i = (int)(max(f, (int64_t)0) / Sk), j = (int)(f - (int64_t)i * Sk);
+    int i = f >= 0 ? (int)(f / Sk) : -(int)((skew + (int64_t)Sk - 1) / Sk), j = (int)(f - (int64_t)i * Sk);
     const int di = 256 * EPC / Sk, dj = 256 * EPC - di * Sk;
     for (; c < cend; c += 256, f += 256 * EPC) {
         float v[EPC];
