@@ -322,7 +322,7 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
     return DIDI_OK;
 }
 
-LaParams make_params(const didi_long_attn_args* a) {
+LaParams make_params(const didi_long_attn_args* a, bool bwd) {
     LaParams p{};
     p.B = a->B; p.H = a->heads; p.Hk = a->kv_heads; p.G = a->heads / a->kv_heads; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D;
     p.HG = a->table ? a->heads : a->kv_heads;
@@ -339,9 +339,10 @@ LaParams make_params(const didi_long_attn_args* a) {
     p.ldq = a->ldq; p.ldk = a->ldk; p.ldv = a->ldv; p.ldo = a->ldo; p.lddo = a->lddo; p.lddq = a->lddq; p.lddk = a->lddk; p.lddv = a->lddv;
     p.lse = a->lse;
     p.table = a->table; p.map = a->buckets; p.nb = a->num_buckets; p.maxd = a->table ? a->max_distance : 0;
-    p.drop_p = a->drop_p;
-    p.inv_keep = a->drop_p > 0.f ? 1.0f / (1.0f - a->drop_p) : 1.f;
     p.thr = (uint32_t)fminf(a->drop_p * 4294967296.0f, 4294967040.0f);
+    const float inv_keep = p.thr ? 1.0f / (1.0f - a->drop_p) : 1.f;
+    p.on = std::min(inv_keep, bwd ? 32768.f : 128.f);
+    p.rest = inv_keep / p.on;
     p.seed = a->seed; p.offset = a->offset;
     return p;
 }
@@ -363,7 +364,7 @@ extern "C" int didi_long_attention_forward(const didi_long_attn_args* a, void* s
     const Plan q = make_plan(a);
     if (q.fwd_bytes && (!a->workspace || a->workspace_bytes < q.fwd_bytes)) return DIDI_ERR_WORKSPACE;
     DIDI_CHECK_ARG((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0);
-    LaParams p = make_params(a);
+    LaParams p = make_params(a, false);
     set_cut(p, q.f);
     p.part = static_cast<float*>(a->workspace);
     p.ml = p.part + (int64_t)q.f.ns * a->B * a->heads * a->Sq * a->D;
@@ -377,7 +378,7 @@ extern "C" int didi_long_attention_backward(const didi_long_attn_args* a, void* 
     const Plan q = make_plan(a);
     if (q.bwd_bytes && (!a->workspace || a->workspace_bytes < q.bwd_bytes)) return DIDI_ERR_WORKSPACE;
     DIDI_CHECK_ARG((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0);
-    LaParams p = make_params(a);
+    LaParams p = make_params(a, true);
     char* ws = static_cast<char*>(a->workspace);
     p.rows = reinterpret_cast<float*>(ws);
     p.part = reinterpret_cast<float*>(ws + q.rows);

@@ -50,7 +50,7 @@ struct LaParams {
     const void* table;  // [nb][H]
     const int32_t* map; // [2 maxd + 1]
     int nb, maxd;
-    float drop_p, inv_keep;
+    float on, rest;  // factors of a kept probability and of the sums over them (drop4)
     uint32_t thr;
     uint64_t seed, offset;
     uint32_t images;  // bytes of LDS before the bias
@@ -476,13 +476,15 @@ __device__ __forceinline__ void bias_fill(const LaParams& p, int head, float* v,
     }
 }
 
-// keep (1 / (1 - p)) or drop (0) of the 4 probabilities of keys j0 .. j0 + 3 (j0 % 4 == 0) of one row: the stream of
-// didi_attention_train_forward: element (b, h, i, j) is dropped iff word j & 3 of Philox(offset + ((b H + h) Sq + i) ceil(Sk / 4) + j / 4) < p 2^32
+// keep (the factor `on`) or drop (0) of the 4 probabilities of keys j0 .. j0 + 3 (j0 % 4 == 0) of one row: the stream of
+// didi_attention_train_forward: element (b, h, i, j) is dropped iff word j & 3 of Philox(offset + ((b H + h) Sq + i) ceil(Sk / 4) + j / 4) < p 2^32.
+// 1 / (1 - p) = on rest: what fp16's range leaves no room for on the 16-bit probabilities -- up to 1 in the backward, up to 2^8 in the forward, whose
+// running maximum lags -- goes onto the fp32 sums.
 __device__ __forceinline__ void drop4(const LaParams& p, uint64_t row, int j0, float k[4]) {
     uint32_t w[4];
     philox4x32_10(p.offset + row * (uint64_t)((p.Sk + 3) >> 2) + (uint64_t)(j0 >> 2), p.seed, w);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = w[e] < p.thr ? 0.f : p.inv_keep;
+    for (int e = 0; e < 4; ++e) k[e] = w[e] < p.thr ? 0.f : p.on;
 }
 
 // Tiles of the contraction in LDS: 32 rows (16 bits, unshared: 64) for each wave that takes a part of them, and as many tiles -- the current one
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     const float m2 = m * mul;  // base-2 maximum
     if constexpr (WK == 1) {
         if (r >= R) return;
-        const float inv = p.ns > 1 ? 1.f : l > 0.f ? 1.f / l : 0.f;
+        const float inv = p.ns > 1 ? 1.f : l > 0.f ? p.rest / l : 0.f;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
                 *reinterpret_cast<float4*>(p.part + ((int64_t)split * rows_all + id) * p.D + d) = make_float4(v[0], v[1], v[2], v[3]);
                 if (d == 0) *reinterpret_cast<float2*>(p.ml + ((int64_t)split * rows_all + id) * 2) = make_float2(top, sum);
             } else {
-                const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                const float inv = sum > 0.f ? p.rest / sum : 0.f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] *= inv;
                 T::store4(p.Ow, (int64_t)b * p.ob + (int64_t)ii * p.ldo + hd * p.D + d, v);
@@ -772,7 +774,7 @@ __global__ void __launch_bounds__(256) la_join(LaParams p) {
         }
     }
     if (row >= rows || d >= p.D) return;
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum > 0.f ? p.rest / sum : 0.f;
     const float out[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
     const int i = (int)(row % p.Sq);
     const int64_t bh = row / p.Sq;
@@ -982,7 +984,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] *= dp[e] - delta;
+                for (int e = 0; e < 16; ++e) s[e] *= fmaf(dp[e], p.rest, -delta);
                 if (BIAS && p.tpart) {
                     if (near) {
                         float* to = skew + (lane & 31) * 63 + 31 + 4 * h;
@@ -1366,7 +1368,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
                 f32x16 ds;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    ds[e] = s[e] * (dp[e] - dl[e]);
+                    ds[e] = s[e] * fmaf(dp[e], p.rest, -dl[e]);
                     if constexpr (T::F16) ds[e] *= fs;
                 }
                 if constexpr (!T::F32) {
@@ -1400,7 +1402,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
                 const int d = dt * 32 + gq * 8 + 4 * h;
                 if (d >= p.D) continue;
                 const float a[4] = {dk[dt][4 * gq] * out, dk[dt][4 * gq + 1] * out, dk[dt][4 * gq + 2] * out, dk[dt][4 * gq + 3] * out};
-                const float c[4] = {dv[dt][4 * gq], dv[dt][4 * gq + 1], dv[dt][4 * gq + 2], dv[dt][4 * gq + 3]};
+                const float c[4] = {dv[dt][4 * gq] * p.rest, dv[dt][4 * gq + 1] * p.rest, dv[dt][4 * gq + 2] * p.rest, dv[dt][4 * gq + 3] * p.rest};
                 write(key, d, a, true);
                 write(key, d, c, false);
             }
@@ -1415,7 +1417,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {
                     const f32x16& x = pass == 0 ? dk[dt] : dv[dt];
-                    const float f = pass == 0 ? out : 1.f;
+                    const float f = pass == 0 ? out : p.rest;
                     *reinterpret_cast<float4*>(ox + (wave * 32 + (lane & 31)) * LD + dt * 32 + gq * 8 + 4 * h) =
                         make_float4(x[4 * gq] * f, x[4 * gq + 1] * f, x[4 * gq + 2] * f, x[4 * gq + 3] * f);
                 }
