@@ -73,6 +73,17 @@ struct E16 {
         *reinterpret_cast<uint2*>(static_cast<u16*>(p[0]) + off) = hi;
         if (p[1]) *reinterpret_cast<uint2*>(static_cast<u16*>(p[1]) + off) = lo;
     }
+    // the attention's output, a mean of the values: beyond fp16's largest number by no more than the 16-bit probabilities may have put it there (2^-11
+    // of it, and fp32's rest), it is that number
+    __device__ static void store4_mean(void* const* p, int64_t off, float v[4]) {
+        if constexpr (F16) {
+            if (fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))) > 65504.f) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fabsf(v[e]) <= 65568.f ? fminf(fmaxf(v[e], -65504.f), 65504.f) : v[e];
+            }
+        }
+        store4(p, off, v);
+    }
     __device__ static float elem(const void* p, int64_t off) { return to_f32(static_cast<const u16*>(p)[off]); }
 };
 struct EF32 {
@@ -82,6 +93,7 @@ struct EF32 {
     __device__ static void store4(void* const* p, int64_t off, const float v[4]) {
         *reinterpret_cast<float4*>(static_cast<float*>(p[0]) + off) = make_float4(v[0], v[1], v[2], v[3]);
     }
+    __device__ static void store4_mean(void* const* p, int64_t off, float v[4]) { store4(p, off, v); }
     __device__ static float elem(const void* p, int64_t off) { return static_cast<const float*>(p)[off]; }
 };
 // ---- LDS images [rows][DP] in 16-byte chunks, XOR-swizzled within a row so that the reads use all 64 banks: 16 neighbouring rows at one chunk
@@ -524,7 +536,6 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     Bias<T> bias;
     if constexpr (BIAS) bias.ask(p, 0, tid);
-    if constexpr (T::F16) f16_saturate_mode();
     const int rt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.HG), hg = (int)blockIdx.x - b * p.HG;
     const int head0 = p.Gr > 1 ? hg * p.Gr : hg, kvh = p.Gr > 1 ? hg : p.G > 1 ? hg / p.G : hg;
     const int R = p.Gr * p.Sq, rbase = rt * C::ROWS, wr = wave / WK, wk = wave % WK, rw = rbase + wr * 32;
@@ -674,9 +685,9 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
             for (int gq = 0; gq < 4; ++gq) {
                 const int d = dt * 32 + gq * 8 + 4 * h;
                 if (d >= p.D) continue;
-                const float v[4] = {o[dt][4 * gq] * inv, o[dt][4 * gq + 1] * inv, o[dt][4 * gq + 2] * inv, o[dt][4 * gq + 3] * inv};
+                float v[4] = {o[dt][4 * gq] * inv, o[dt][4 * gq + 1] * inv, o[dt][4 * gq + 2] * inv, o[dt][4 * gq + 3] * inv};
                 if (p.ns > 1) *reinterpret_cast<float4*>(p.part + ((int64_t)split * rows_all + rowid) * p.D + d) = make_float4(v[0], v[1], v[2], v[3]);
-                else T::store4(p.Ow, (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D + d, v);
+                else T::store4_mean(p.Ow, (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D + d, v);
             }
         if (h == 0) {
             if (p.ns > 1) *reinterpret_cast<float2*>(p.ml + ((int64_t)split * rows_all + rowid) * 2) = make_float2(m2, l);
@@ -725,7 +736,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
                 const float inv = sum > 0.f ? p.rest / sum : 0.f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] *= inv;
-                T::store4(p.Ow, (int64_t)b * p.ob + (int64_t)ii * p.ldo + hd * p.D + d, v);
+                T::store4_mean(p.Ow, (int64_t)b * p.ob + (int64_t)ii * p.ldo + hd * p.D + d, v);
                 if (d == 0 && p.lse) p.lse[id] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
             }
         }
@@ -775,21 +786,25 @@ __global__ void __launch_bounds__(256) la_join(LaParams p) {
     }
     if (row >= rows || d >= p.D) return;
     const float inv = sum > 0.f ? p.rest / sum : 0.f;
-    const float out[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    float out[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
     const int i = (int)(row % p.Sq);
     const int64_t bh = row / p.Sq;
-    T::store4(p.Ow, bh / p.H * p.ob + (int64_t)i * p.ldo + bh % p.H * p.D + d, out);
+    T::store4_mean(p.Ow, bh / p.H * p.ob + (int64_t)i * p.ldo + bh % p.H * p.D + d, out);
     if (d == 0 && p.lse) p.lse[row] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
 }
 
 // ------------------------------------------------------------------ backward: dQ, D = do . o, and the sums of ds by distance
-// fp16: ds is scaled by a power of two before it is rounded to 16 bits, so that small gradients keep their bits: 64 / |do_i| per row here
-// (undone at the end: the lane owns the row), 64 / max_i |do_i| of the head in la_backward_kv.  |ds| <= 2 |do| max|v|, so nothing
-// saturates below |v| = 512, and probabilities down to 1e-6 of a row stay normal numbers.
-__device__ __forceinline__ float pow2_scale(float norm) {
+// fp16: ds is scaled by a power of two before it is rounded to 16 bits, so that small gradients keep their bits and none overflows.  Here it
+// belongs to a row (undone at the end: the lane owns the row): 32 .. 64 / |do_i| at first, which keeps probabilities down to 1e-6 of a row normal
+// numbers, and less from the first block on whose score gradients would leave the range.  In la_backward_kv it belongs to a key, and what bounds
+// its gradients is known beforehand: |ds_ij| <= max_i |do_i| |v_j| / (1 - drop_p) + max_i |do_i . o_i| is brought to 2^14 .. 2^15.  Results that
+// lie beyond fp16 are infinite, as any rounding to fp16 makes them (a loss scaler looks for that).  Watching the gradients costs nothing without a
+// bias (8 x 12 heads of 64, 512 x 512: the backward 48 us with and without) and 4 of 79 us with one, whose sums want them unscaled.
+// the power of two that brings norm into [2^to, 2^(to + 1)); 1 if there is none
+__device__ __forceinline__ float pow2_scale(float norm, int to) {
     if (!(norm > 0.f) || !(norm < INFINITY)) return 1.f;
     const int e = (int)((__builtin_bit_cast(uint32_t, norm) >> 23) & 0xff) - 127;  // norm >= 2^e
-    return __builtin_bit_cast(float, (uint32_t)(127 + min(max(5 - e, -100), 100)) << 23);
+    return __builtin_bit_cast(float, (uint32_t)(127 + min(max(to - e, -100), 100)) << 23);
 }
 
 // Bound by the products: 2 x 16 heads of 128, 2048 x 8192, bf16: 375 us for its three, 916 TFLOP/s.  Short ones by latency: causal fp32 128 x 128,
@@ -821,7 +836,6 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     Bias<T> bias;
     if constexpr (BIAS) bias.ask(p, 0, tid);
-    if constexpr (T::F16) f16_saturate_mode();
     const int rt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.HG), hg = (int)blockIdx.x - b * p.HG;
     const int head0 = p.Gr > 1 ? hg * p.Gr : hg, kvh = p.Gr > 1 ? hg : p.G > 1 ? hg / p.G : hg;
     const int R = p.Gr * p.Sq, rbase = rt * C::ROWS, wk = wave % WK, rw = rbase + wave / WK * 32;
@@ -896,7 +910,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
         norm += __shfl_xor(norm, 32, 64);
     }
     norm = __builtin_amdgcn_sqrtf(norm);
-    const float fs = T::F16 ? pow2_scale(norm) : 1.f;
+    float fs = T::F16 ? pow2_scale(norm, 5) : 1.f;
     const float sub = lse == -INFINITY ? -INFINITY : -lse * LOG2E;  // a row that sees nothing: p = exp2(-inf) = 0
     if (split == 0 && wk == 0 && rok && h == 0) {  // for la_backward_kv
         const int64_t rows_all = (int64_t)p.B * p.H * p.Sq;
@@ -983,8 +997,29 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
                         for (int e = 0; e < 4; ++e) dp[4 * gq + e] *= k[e];
                     }
                 }
+                const float ds_scale = T::F16 && !BIAS ? fs : 1.f;  // a bias wants its sums unscaled
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] *= fmaf(dp[e], p.rest, -delta);
+                for (int e = 0; e < 16; ++e) s[e] *= fmaf(dp[e], p.rest * ds_scale, -delta * ds_scale);
+                if constexpr (T::F16) {
+                    const float rest_scale = BIAS ? fs : 1.f;
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
+                    if (__any(top * rest_scale > 49152.f)) {
+                        asm volatile("");
+                        top = max_halves(top) * rest_scale;  // both halves of a row keep one scale
+                        const float less = top > 49152.f && top < INFINITY ? pow2_scale(top, 12) : 1.f;
+#pragma unroll
+                        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) dq[dt][e] *= less;
+                        if constexpr (!BIAS) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) s[e] *= less;
+                        }
+                        fs *= less;
+                    }
+                }
                 if (BIAS && p.tpart) {
                     if (near) {
                         float* to = skew + (lane & 31) * 63 + 31 + 4 * h;
@@ -1003,7 +1038,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
                         else far_r += sum;
                     }
                 }
-                if constexpr (T::F16) {
+                if constexpr (T::F16 && BIAS) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[e] *= fs;
                 }
@@ -1181,7 +1216,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     using C = BwdKCfg<T, DP, WQ>;
     using QT = Tile<T, DP, C::BQ>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ float top4[4];
+    __shared__ float top4[2][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     if constexpr (BIAS) {
         if ((int)blockIdx.x >= p.B * p.Hk) {
@@ -1192,7 +1227,6 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     }
     Bias<T> bias;
     if constexpr (BIAS) bias.ask(p, 0, tid);
-    if constexpr (T::F16) f16_saturate_mode();
     const int kt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.Hk), kvh = (int)blockIdx.x - b * p.Hk;
     const int kbase = kt * C::KEYS, wq = wave % WQ, kw = kbase + wave / WQ * 32, key = kw + (lane & 31);
     const int kend = visible_end(p, b);
@@ -1237,21 +1271,38 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     int blo = 0, bhi = -1;
     if constexpr (BIAS) bias.finish(p, kvh * p.G + gcur, bv, reinterpret_cast<int*>(bv + len), tid, blo, bhi);
     float fs = 1.f;
+    const bool vis = seen != 0;
     if constexpr (T::F16) {
-        float top = 0.f;
-        const float* norms = p.rows + 2 * rows_all + ((int64_t)b * p.H + kvh * p.G) * p.Sq;
+        float top[2] = {0.f, 0.f};  // of D and of |do|
+        const float* of = p.rows + rows_all + ((int64_t)b * p.H + kvh * p.G) * p.Sq;
         const int n = p.G * p.Sq;
         for (int x = tid; x < n; x += 1024)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top = fmaxf(top, norms[min(x + 256 * k, n - 1)]);
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        if (lane == 0) top4[wave] = top;
+                for (int w = 0; w < 2; ++w) top[w] = fmaxf(top[w], fabsf(of[w * rows_all + min(x + 256 * k, n - 1)]));
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) top[w] = fmaxf(top[w], __shfl_xor(top[w], o, 64));
+            if (lane == 0) top4[w][wave] = top[w];
+        }
         barrier();
-        fs = pow2_scale(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
+#pragma unroll
+        for (int w = 0; w < 2; ++w) top[w] = fmaxf(fmaxf(top4[w][0], top4[w][1]), fmaxf(top4[w][2], top4[w][3]));
+        float vv = 0.f;  // |v_j|^2: a masked key's gradients are zeros, whatever the scale
+#pragma unroll
+        for (int c = 0; c < Frag<T, DP>::N; ++c) {
+            const uint32_t a[4] = {vf.x[c].x, vf.x[c].y, vf.x[c].z, vf.x[c].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float e0 = T::to_f32((u16)a[k]), e1 = T::to_f32((u16)(a[k] >> 16));
+                vv = fmaf(e0, e0, fmaf(e1, e1, vv));
+            }
+        }
+        vv += __shfl_xor(vv, 32, 64);
+        fs = pow2_scale(fmaf(top[1] * __builtin_amdgcn_sqrtf(vv), p.on * p.rest, top[0]), 14);
     }
-
-    const bool vis = seen != 0;
     if (!vis) {  // whatever a masked key holds, it is not multiplied
         kf.clear();
         vf.clear();

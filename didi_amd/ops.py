@@ -810,7 +810,7 @@ def cross_attention_backward(q, k, v, o, saved, dO, heads, kv_heads=None, causal
                              rel_bias=None, drop_p=0.0, seed=0, offset=0, out=None):
     """Backward of ``cross_attention(..., need_grad=True)`` with the same arguments -> (dq, dk, dv), and dtable where a bias was given.
     ``out`` = (dq, dk, dv): views to write into (e.g. the thirds of a fused projection's gradient), not over operands; default fresh
-    contiguous tensors.
+    contiguous tensors.  fp16: gradients beyond the type's range are infinite, as a loss scaler expects.
     Deterministic."""
     before, after = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
     dev, dt, shape, kv_shape = q.device, q.dtype, q.shape, k.shape

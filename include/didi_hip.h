@@ -697,6 +697,7 @@ int didi_train_target_backward(const float* x0hat, const float* emb, const float
  * A row that sees no key gives o = 0, lse = -inf and no gradients (didi_attention's rows without a visible key average all values
  * instead); keys and values that are not visible to a dialog are never multiplied, whatever they hold.  Statistics and sums are fp32.
  * dtype BF16 / FP16: one product per pair, probabilities and score gradients rounded to that type; FP32: fp32 products throughout.
+ * FP16 score gradients are scaled by powers of two so that none overflows on the way; a result beyond the type's range is infinite.
  * O_lo (BF16 / FP16, optional): the output's remainder plane; the backward adds it to O where it is given: every score gradient holds D = do . o.
  * Strides in elements: ld* between rows, *_batch between dialogs (inputs may repeat a dialog with 0).
  * 16-byte aligned bases and strides.  D % 8 == 0 (FP32: % 4), D <= 128; max_distance <= 512, num_buckets <= 1024.

@@ -71,3 +71,61 @@ def test_the_highest_dropout_over_one_key(ops, dtype):  # noqa: F811
     n24 = 64 * 2.0 ** -24
     assert ((o.double()[0] - want_o).abs() <= (U[dtype] + n24) * want_o.abs() + SUB[dtype]).all()
     assert ((dv.double()[0, 0] - want_dv).abs() <= U[dtype] * want_dv.abs() + n24 * (keep * do.double()[0].abs()).sum(0) + SUB[dtype]).all()
+
+
+@pytest.mark.parametrize("drop_p", [0.0, 0.5, 0.9])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D,bias", [(2, 2, 2, 70, 8, 128, False), (1, 4, 2, 130, 40, 64, False), (2, 3, 1, 1, 5, 96, False), (1, 2, 2, 400, 5, 128, False),
+                                                 (1, 4, 2, 130, 40, 64, True), (2, 2, 2, 70, 300, 32, True), (24, 16, 16, 130, 6, 64, False)])
+def test_large_values_and_gradients_along_them(ops, dtype, B, H, Hk, Sq, Sk, D, bias, drop_p):  # noqa: F811
+    """Value rows of norm 1000 to 4000 and do along one of them: score gradients that overflow fp16 unless they are scaled by their own size."""
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=Sq + Sk, scale_q=2.0 ** -4)
+    v.mul_(200 if D > 64 else 400)
+    along = v.reshape(B, Sk, Hk, D)[:, torch.arange(Sq, device="cuda") % Sk] / 400  # [B, Sq, Hk, D]
+    do.copy_(along.repeat_interleave(H // Hk, 2).reshape(B, Sq, H * D))
+    kw = dict(drop_p=drop_p, seed=3)
+    keep = keep_of(B, H, Sq, Sk, drop_p, 3) if drop_p else None
+    ref = {}
+    if bias:
+        table = torch.randn(32, H, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
+        ref["rel_bias"] = kw["rel_bias"] = (table, ops.relative_buckets())
+    got, _ = run(ops, q, k, v, do, H, Hk, **kw)
+    val, tol = reference(q, k, v, do, H, Hk, dtype, keep=keep, **ref)
+    assert all(float(x.abs().max()) < 60000 for n, x in val.items() if n != "lse")
+    compare(got, val, tol)
+
+
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 1, 64), (200, 3, 64), (300, 70, 128), (40, 300, 32)])
+def test_fp16_results_beyond_the_range_are_infinite(ops, Sq, Sk, D):  # noqa: F811
+    """What overflows fp16 is infinite -- what a loss scaler looks for -- and the rest is right."""
+    B, H = 2, 3
+    q, k, v, do = make(B, H, H, Sq, Sk, D, "fp16", seed=8)
+    do.mul_(14000)
+    k.mul_(2.0)
+    v.mul_(2.0)
+    kw = dict(drop_p=0.5, seed=9)
+    keep = keep_of(B, H, Sq, Sk, 0.5, 9)
+    got, _ = run(ops, q, k, v, do, H, H, **kw)
+    val, tol = reference(q, k, v, do, H, H, "fp16", keep=keep)
+    beyond = 0
+    for n, x in got.items():
+        out, within = val[n].abs() - tol[n] > 65520, val[n].abs() + tol[n] < 65504
+        beyond += int(out.sum())
+        assert torch.equal(x.double()[out], torch.where(val[n] > 0, math.inf, -math.inf)[out]), n
+        assert ((x.double() - val[n]).abs() <= tol[n])[within].all(), n
+    assert beyond or Sk == 1 and Sq == 1
+    v.fill_(40000.0)
+    o = ops.cross_attention(q, k, v, H, **kw)  # half of the probabilities count twice
+    want = (torch.softmax((q.double().reshape(B, Sq, H, D).transpose(1, 2) @ k.double().reshape(B, Sk, H, D).permute(0, 2, 3, 1)) / math.sqrt(D), -1) * keep).sum(-1) * 40000
+    want = want.transpose(1, 2)[..., None].expand(B, Sq, H, D).reshape(B, Sq, H * D)
+    assert torch.isinf(o[want > 65520 * 1.001]).all() and torch.isfinite(o[want < 65504 / 1.001]).all()
+
+
+@pytest.mark.parametrize("Sq,Sk", [(1, 300), (1, 5000), (40, 300), (300, 1000), (200, 3)])
+def test_fp16_values_at_the_largest_number(ops, Sq, Sk):  # noqa: F811
+    """A mean of the largest number is that number: the 16-bit probabilities' roundings do not carry it over."""
+    q, k, v, _ = make(2, 3, 3, Sq, Sk, 64, "fp16", seed=2)
+    for sign in (1.0, -1.0):
+        o = ops.cross_attention(q, k, torch.full_like(v, sign * 65504.0), 3)
+        # probabilities rounded once, and fp32's rest of Sk terms
+        assert ((o.double() - sign * 65504.0).abs() <= 65504.0 * (2 * 2.0 ** -11 + Sk * 2.0 ** -24)).all()
