@@ -678,20 +678,22 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     const float m2 = m * mul;  // base-2 maximum
     if constexpr (WK == 1) {
         if (r >= R) return;
-        const float inv = p.ns > 1 ? 1.f : l > 0.f ? p.rest / l : 0.f;
+        const float inv = p.ns > 1 ? 1.f : p.rest / l;  // only l == 0 has seen nothing: a sum that is not a number stays one, and so does the row
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
             for (int gq = 0; gq < 4; ++gq) {
                 const int d = dt * 32 + gq * 8 + 4 * h;
                 if (d >= p.D) continue;
-                float v[4] = {o[dt][4 * gq] * inv, o[dt][4 * gq + 1] * inv, o[dt][4 * gq + 2] * inv, o[dt][4 * gq + 3] * inv};
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = l == 0.f ? 0.f : o[dt][4 * gq + e] * inv;
                 if (p.ns > 1) *reinterpret_cast<float4*>(p.part + ((int64_t)split * rows_all + rowid) * p.D + d) = make_float4(v[0], v[1], v[2], v[3]);
                 else T::store4_mean(p.Ow, (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D + d, v);
             }
         if (h == 0) {
             if (p.ns > 1) *reinterpret_cast<float2*>(p.ml + ((int64_t)split * rows_all + rowid) * 2) = make_float2(m2, l);
-            else if (p.lse) p.lse[rowid] = l > 0.f ? (m2 + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+            else if (p.lse) p.lse[rowid] = l == 0.f ? -INFINITY : (m2 + __builtin_amdgcn_logf(l)) * LN2;
         }
     } else {
         // join the waves of a row group: O^T to LDS as [wave][row][d], maxima and sums beside it
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
 #pragma unroll
             for (int k = 0; k < WK; ++k) {
                 const float2 e = mx[w0 + k * 32];
-                if (!(e.y > 0.f)) continue;
+                if (e.y == 0.f) continue;  // saw nothing; a sum that is not a number is not left out
                 const float a = __builtin_amdgcn_exp2f(e.x - top);
                 sum += a * e.y;
                 const float4 ov = *reinterpret_cast<const float4*>(ox + (w0 + k * 32) * LD + d);
@@ -733,11 +735,11 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
                 *reinterpret_cast<float4*>(p.part + ((int64_t)split * rows_all + id) * p.D + d) = make_float4(v[0], v[1], v[2], v[3]);
                 if (d == 0) *reinterpret_cast<float2*>(p.ml + ((int64_t)split * rows_all + id) * 2) = make_float2(top, sum);
             } else {
-                const float inv = sum > 0.f ? p.rest / sum : 0.f;
+                const float inv = sum == 0.f ? 0.f : p.rest / sum;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] *= inv;
                 T::store4_mean(p.Ow, (int64_t)b * p.ob + (int64_t)ii * p.ldo + hd * p.D + d, v);
-                if (d == 0 && p.lse) p.lse[id] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
+                if (d == 0 && p.lse) p.lse[id] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
             }
         }
     }
@@ -761,7 +763,7 @@ __global__ void __launch_bounds__(256) la_join(LaParams p) {
         for (int s = sl; s < p.ns; s += SL) {
             const float2 e = reinterpret_cast<const float2*>(p.ml)[s * rows + row];
             const float4 o = d < p.D ? *reinterpret_cast<const float4*>(p.part + (s * rows + row) * p.D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float a = e.y > 0.f ? __builtin_amdgcn_exp2f(e.x - top) : 0.f;  // a split that saw nothing wrote zeros and -inf
+            const float a = e.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(e.x - top);  // a split that saw nothing wrote zeros and -inf
             sum = fmaf(a, e.y, sum);
             v.x = fmaf(a, o.x, v.x);
             v.y = fmaf(a, o.y, v.y);
@@ -785,12 +787,12 @@ __global__ void __launch_bounds__(256) la_join(LaParams p) {
         }
     }
     if (row >= rows || d >= p.D) return;
-    const float inv = sum > 0.f ? p.rest / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : p.rest / sum;
     float out[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
     const int i = (int)(row % p.Sq);
     const int64_t bh = row / p.Sq;
     T::store4_mean(p.Ow, bh / p.H * p.ob + (int64_t)i * p.ldo + bh % p.H * p.D + d, out);
-    if (d == 0 && p.lse) p.lse[row] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
+    if (d == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
 // ------------------------------------------------------------------ backward: dQ, D = do . o, and the sums of ds by distance

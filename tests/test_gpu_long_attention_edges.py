@@ -129,3 +129,70 @@ def test_fp16_values_at_the_largest_number(ops, Sq, Sk):  # noqa: F811
         o = ops.cross_attention(q, k, torch.full_like(v, sign * 65504.0), 3)
         # probabilities rounded once, and fp32's rest of Sk terms
         assert ((o.double() - sign * 65504.0).abs() <= 65504.0 * (2 * 2.0 ** -11 + Sk * 2.0 ** -24)).all()
+
+
+def cuts(Sq):
+    """Sizes at which the launches are cut differently: 4 / 2 / 1 row blocks a workgroup, one and several splits of the keys."""
+    return {1: [(3, 4, 2, 300, 64), (1, 2, 2, 5000, 128)], 40: [(3, 4, 2, 300, 64), (1, 1, 1, 3000, 96)], 200: [(3, 4, 2, 300, 64), (24, 12, 12, 130, 32)],
+            300: [(24, 8, 8, 130, 64)]}[Sq]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Sq,size", [(s, c) for s in (1, 40, 200, 300) for c in cuts(s)])
+def test_nan_and_infinity_at_visible_places_reach_the_result(ops, dtype, Sq, size):  # noqa: F811
+    """A query or a visible key that holds NaN gives rows of NaN and gradients of NaN, +inf scores do, whatever the launch's cut, and the other rows,
+    heads and dialogs keep their bits."""
+    B, H, Hk, Sk, D = size
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=Sq)
+    G, b, row, key, kh = H // Hk, B // 2, Sq // 2, Sk * 2 // 3, Hk - 1
+    count = torch.full((B,), Sk, dtype=torch.int32, device="cuda")
+    count[0] = key + 1
+    cut = lambda x, n: x.reshape(x.shape[0], x.shape[1], n, D)  # noqa: E731
+    clean, clean_lse = run(ops, q, k, v, do, H, Hk, key_count=count)
+    same = torch.ones(B, Sq, H, dtype=torch.bool, device="cuda")
+
+    def check(hit, got, lse):
+        o = cut(got["o"], H)
+        assert torch.isnan(o[hit]).all() and torch.isnan(lse.transpose(1, 2)[hit]).all()
+        assert torch.equal(o[same & ~hit], cut(clean["o"], H)[same & ~hit]) and torch.equal(lse.transpose(1, 2)[same & ~hit], clean_lse.transpose(1, 2)[same & ~hit])
+        assert torch.isnan(cut(got["dq"], H)[hit]).all()
+        visible = torch.arange(Sk, device="cuda")[None, :] < count[:, None]
+        dead = hit.any(1).reshape(B, Hk, G).any(2)[:, None, :] & visible[:, :, None]  # every visible key of a head gets a part of each row
+        for n in ("dk", "dv"):
+            assert torch.isnan(cut(got[n], Hk)[dead]).all(), n
+
+    x = q.clone()
+    cut(x, H)[b, row, H - 1, 5] = math.nan
+    hit = torch.zeros_like(same)
+    hit[b, row, H - 1] = True
+    check(hit, *run(ops, x, k, v, do, H, Hk, key_count=count))
+    for bad in (math.nan, math.inf):
+        x = k.clone()
+        cut(x, Hk)[b, key, kh, 3] = bad
+        hit = torch.zeros_like(same)
+        up = cut(q, H)[b, :, kh * G:, 3] > 0  # -inf scores otherwise: a key of no weight
+        hit[b, :, kh * G:] = True if math.isnan(bad) else up
+        same = torch.ones_like(same)
+        same[b, :, kh * G:] = False
+        check(hit, *run(ops, q, x, v, do, H, Hk, key_count=count))
+        x = v.clone()
+        cut(x, Hk)[b, key, kh, 3] = bad
+        got = cut(ops.cross_attention(q, k, x, H, kv_heads=Hk, key_count=count, need_grad=True)[0], H)
+        assert not torch.isfinite(got[b, :, kh * G:, 3]).any()
+        got[b, :, kh * G:, 3] = cut(clean["o"], H)[b, :, kh * G:, 3]
+        assert torch.equal(got, cut(clean["o"], H))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Sq", [1, 40, 200])
+def test_a_bucket_outside_the_table_is_nan_in_the_attention(ops, dtype, Sq):  # noqa: F811
+    B, H, Sk, D = 2, 3, 300, 64
+    q, k, v, do = make(B, H, H, Sq, Sk, D, dtype, seed=1)
+    table = torch.randn(32, H, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
+    for at, value in ((20, 32), (-17, -1), (128, 1 << 30), (-128, 32)):
+        buckets = ops.relative_buckets(32, 128)
+        buckets[128 + at] = value
+        rel = (torch.arange(Sk)[None] - torch.arange(Sq)[:, None] - 100).clamp(-128, 128)
+        hit = (rel == at).any(1).cuda()
+        o = ops.cross_attention(q, k, v, H, scale=0.125, q_start=100, rel_bias=(table, buckets))
+        assert torch.isnan(o[:, hit]).all() and torch.isfinite(o[:, ~hit]).all()
