@@ -1231,7 +1231,8 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     if constexpr (BIAS) bias.ask(p, 0, tid);
     const int kt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.Hk), kvh = (int)blockIdx.x - b * p.Hk;
     const int kbase = kt * C::KEYS, wq = wave % WQ, kw = kbase + wave / WQ * 32, key = kw + (lane & 31);
-    const int kend = visible_end(p, b);
+    int kend = visible_end(p, b);
+    if (p.causal) kend = min(kend, p.q_start + p.Sq);  // the last row's position: what lies behind it is visible to no row
     const int seen = key < kend ? p.mask ? p.mask[(int64_t)b * p.Sk + key] : 1 : 0;
     const int64_t kvrow = (int64_t)b * p.kb + (int64_t)key * p.ldk + kvh * p.D, vrow = (int64_t)b * p.vb + (int64_t)key * p.ldv + kvh * p.D;
     const int64_t rows_all = (int64_t)p.B * p.H * p.Sq;

@@ -196,3 +196,25 @@ def test_a_bucket_outside_the_table_is_nan_in_the_attention(ops, dtype, Sq):  # 
         hit = (rel == at).any(1).cuda()
         o = ops.cross_attention(q, k, v, H, scale=0.125, q_start=100, rel_bias=(table, buckets))
         assert torch.isnan(o[:, hit]).all() and torch.isfinite(o[:, ~hit]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Sq,q_start,Sk,D,bias", [(1, 0, 40, 64, False), (7, 20, 60, 32, False), (40, 10, 300, 64, True), (200, 0, 230, 128, False), (33, 3, 37, 64, False),
+                                                  (130, 6, 140, 96, True)])
+def test_keys_behind_the_last_query_are_never_used(ops, dtype, Sq, q_start, Sk, D, bias):  # noqa: F811
+    """Causal: a key past position q_start + Sq - 1 is visible to no row."""
+    B, H, Hk = 2, 4, 2
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=6)
+    kw = dict(causal=True, q_start=q_start)
+    if bias:
+        kw["rel_bias"] = (torch.randn(32, H, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda(), ops.relative_buckets(bidirectional=False))
+    for mask in ({}, masks("count", B, Sk), masks("mask", B, Sk)):
+        clean = run(ops, q, k, v, do, H, Hk, **kw, **mask)
+        for bad in (math.nan, math.inf, -math.inf, torch.finfo(DT[dtype]).max):
+            x, y = k.clone(), v.clone()
+            x[:, q_start + Sq:] = bad
+            y[:, q_start + Sq:] = bad
+            got = run(ops, q, x, y, do, H, Hk, **kw, **mask)
+            for n in clean[0]:
+                assert torch.equal(clean[0][n], got[0][n]), (n, bad)
+            assert (got[0]["dk"][:, q_start + Sq:] == 0).all() and (got[0]["dv"][:, q_start + Sq:] == 0).all()
