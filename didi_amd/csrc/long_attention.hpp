@@ -7,8 +7,9 @@
 //   o_i   = sum_j drop(p_ij) v_j           lse_i = log sum_j exp(t_ij)
 //   ds_ij = p_ij (drop(do_i . v_j) - do_i . o_i)
 //   dq_i  = scale sum_j ds_ij k_j     dk_j = scale sum_i ds_ij q_i     dv_j = sum_i drop(p_ij) do_i     dtable[t][h] = sum of ds of bucket t
-// A row that sees no key gives o = 0, lse = -inf and no gradients; keys and values that are not visible to a dialog are never
-// multiplied (their LDS rows are zeros), so whatever lies there -- infinities, NaN -- stays there.
+// A row that sees no key gives o = 0, lse = -inf and no gradients, whatever its query and its do hold; keys and values that no row of a dialog
+// sees are never multiplied (their LDS rows are zeros), so whatever lies there -- infinities, NaN -- stays there.  What the causal limit hides from
+// some rows only is multiplied by zeros for those, as in the products' plain form: it has to be finite.
 //
 // One online softmax pass (running maximum and sum per row, fp32).  Everything is laid out so that one lane owns one row's statistics:
 //   S^T = K Q^T   v_mfma_f32_32x32x16 (32x32x2 in fp32), A = K rows out of LDS, B = Q rows in registers
@@ -861,6 +862,12 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     go.load(p.dO, (int64_t)b * p.dob + (int64_t)i * p.lddo + head * p.D, rok, p.D, h);
     o.load(p.O[0], oo, rok, p.D, h);
     const float lse = rok ? p.lse[rowid] : -INFINITY;
+    if (__any(lse == -INFINITY)) {  // rows that saw nothing: whatever their gradient holds, it is not multiplied
+        if (lse == -INFINITY) {
+            go.clear();
+            o.clear();
+        }
+    }
 
     const int64_t kbase = (int64_t)b * p.kb + kvh * p.D, vbase = (int64_t)b * p.vb + kvh * p.D;
     KV tk, tv;
@@ -898,7 +905,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
         }
         if constexpr (!T::F32) {
             if (p.O[1]) {  // the output's remainder: the sums of ds by distance cancel, so D wants more than the output's 8 or 11 bits
-                o.load(p.O[1], oo, rok, p.D, h);
+                o.load(p.O[1], oo, lse != -INFINITY, p.D, h);
 #pragma unroll
                 for (int c = 0; c < Frag<T, DP>::N; ++c) {
                     const uint32_t a[4] = {o.x[c].x, o.x[c].y, o.x[c].z, o.x[c].w}, e[4] = {go.x[c].x, go.x[c].y, go.x[c].z, go.x[c].w};
@@ -1325,6 +1332,19 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         if (t + C::NS - 1 < t1) issue(t + C::NS - 1);
         const char *Qs = smem + (t - t0) % C::NS * (2 * C::IMG + C::STAT), *Gs = Qs + C::IMG;
         const float* rc = reinterpret_cast<const float*>(Gs + C::IMG + wave * 512);  // -lse log2(e) of the wave's rows, 64 on D
+        // rows that saw nothing are not multiplied either (their constants D and |do| are zeros): a wave clears what it is about to read itself, others
+        // that read the same rows do so too
+        if (uint64_t none = __ballot(rc[lane & (32 * C::NT - 1)] == -INFINITY) & (C::NT == 2 ? ~0ull : 0xffffffffull)) {
+            constexpr int CH = DP / T::EPC;
+            char* at = smem + (Qs - smem) + qrow * CH * 16 + lane * 16;
+            for (; none; none &= none - 1)
+                if (lane < CH) {
+                    const int to = __builtin_ctzll(none) * CH * 16;
+                    *reinterpret_cast<uint4*>(at + to) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(at + to + C::IMG) = make_uint4(0, 0, 0, 0);
+                }
+            asm volatile("" ::: "memory");
+        }
         // a wave none of whose keys is seen by the tile's last row has nothing to add
         if (!p.causal || kw <= p.q_start + min(i0 + qrow + 32 * C::NT, p.Sq) - 1) {
             constexpr int UNROLL = DP > 64 ? 1 : C::NT;
@@ -1437,6 +1457,15 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
                 add<T, DP>(cq, ds, dk);
             }
         }
+    }
+    if (!__all(vis)) {  // keys that nobody saw: nothing, whatever the queries and their gradients hold
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                dk[dt][e] = vis ? dk[dt][e] : 0.f;
+                dv[dt][e] = vis ? dv[dt][e] : 0.f;
+            }
     }
     const float out = p.scale / fs;
     void *dkp[2] = {p.dK, nullptr}, *dvp[2] = {p.dV, nullptr};

@@ -785,7 +785,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_
     bf16, fp16 or fp32, all operands alike; views with strides between rows and dialogs are fine (16-byte aligned).  Head dims up to 128,
     multiples of 8 (fp32: 4).  ``kv_heads``: each key head serves heads / kv_heads query heads.  A key is visible where
     ``key_mask`` int32 [B, Sk] is not 0, before ``key_count`` int32 [B], and (``causal``) up to position q_start + i; a row that sees none
-    gives zeros, and what lies at invisible keys is never used.  ``scale``: default 1/sqrt(D).  ``rel_bias`` = (table [num_buckets, heads],
+    gives zeros, and what lies at keys that no row of a dialog sees is never used.  ``scale``: default 1/sqrt(D).  ``rel_bias`` = (table [num_buckets, heads],
     relative_buckets(...)): a learned bias by the distance from query q_start + i to the key, added to the scaled scores.  ``drop_p``,
     ``seed``, ``offset``: dropout of the probabilities, ``attention_train``'s mask.
     ``need_grad``: -> (o, saved) for ``cross_attention_backward``.  ``out``: written to (a view as for q, not over an operand)."""

@@ -695,7 +695,10 @@ int didi_train_target_backward(const float* x0hat, const float* emb, const float
  *   visible(b, i, j) = j < key_count[b] and key_mask[b, j] != 0 and (not causal or j <= q_start + i)
  *   o_i = sum_j p_ij v_j,  p = dropout(softmax_j(scale q_i . k_j + table[buckets[clamp(j - q_start - i)]][head])) over the visible j
  * A row that sees no key gives o = 0, lse = -inf and no gradients (didi_attention's rows without a visible key average all values
- * instead); keys and values that are not visible to a dialog are never multiplied, whatever they hold.  Statistics and sums are fp32.
+ * instead), whatever its q and do hold; keys and values that no row of their dialog sees are never multiplied, whatever they hold, and get gradients
+ * of 0.  What causal hides from some rows only has to be finite.  NaN at visible places reaches o, lse and the gradients.
+ * A table entry of -inf hides its distances, and so does one below -2.36e38 (scores are kept in base 2).  Statistics and sums are fp32: the backward's
+ * probabilities are right to |lse| 2^-23, so what is to be hidden belongs in key_mask or at -inf, not at a large negative number.
  * dtype BF16 / FP16: one product per pair, probabilities and score gradients rounded to that type; FP32: fp32 products throughout.
  * FP16 score gradients are scaled by powers of two so that none overflows on the way; a result beyond the type's range is infinite.
  * O_lo (BF16 / FP16, optional): the output's remainder plane; the backward adds it to O where it is given: every score gradient holds D = do . o.

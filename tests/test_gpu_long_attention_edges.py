@@ -218,3 +218,81 @@ def test_keys_behind_the_last_query_are_never_used(ops, dtype, Sq, q_start, Sk, 
             for n in clean[0]:
                 assert torch.equal(clean[0][n], got[0][n]), (n, bad)
             assert (got[0]["dk"][:, q_start + Sq:] == 0).all() and (got[0]["dv"][:, q_start + Sq:] == 0).all()
+
+
+def without(x, hit):
+    return torch.where(hit.reshape(hit.shape + (1,) * (x.dim() - hit.dim())), torch.zeros((), dtype=x.dtype, device=x.device), x)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D,q_start,bias", [(3, 4, 2, 70, 100, 64, 30, False), (3, 2, 2, 260, 260, 32, 0, False), (3, 3, 3, 40, 200, 96, 100, True),
+                                                         (24, 8, 8, 130, 130, 64, 0, False), (3, 2, 1, 150, 150, 128, 0, True), (3, 6, 2, 9, 40, 40, 3, False)])
+def test_rows_that_see_nothing_pass_nothing_on(ops, dtype, B, H, Hk, Sq, Sk, D, q_start, bias):  # noqa: F811
+    """Left padding under a causal limit: the padded rows see no key.  Whatever their queries and their gradients hold, their results are zeros and
+    everything else keeps its bits; an empty dialog likewise."""
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=13)
+    pad = torch.arange(B) * 37 % (Sq * 3 // 4) + q_start  # first visible key
+    pad[0], pad[B - 1] = Sk // 3, Sk
+    mask = (torch.arange(Sk)[None] >= pad[:, None]).to(torch.int32).cuda()
+    blind = (torch.arange(Sq)[None] + q_start < pad[:, None]).cuda()  # [B, Sq]
+    kw = dict(causal=True, q_start=q_start, key_mask=mask)
+    if bias:
+        kw["rel_bias"] = (torch.randn(32, H, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda(), ops.relative_buckets(bidirectional=False))
+    clean, lse = run(ops, without(q, blind), k, v, without(do, blind), H, Hk, **kw)
+    assert (lse.transpose(1, 2)[blind] == -math.inf).all()
+    compare(clean, *reference(without(q, blind), k, v, without(do, blind), H, Hk, dtype, **kw))
+    for bad in (math.nan, math.inf, torch.finfo(DT[dtype]).max):
+        x, g = q.clone(), do.clone()
+        x[blind] = bad
+        g[blind] = bad
+        got, again = run(ops, x, k, v, g, H, Hk, **kw)
+        assert torch.equal(lse, again)
+        for n in clean:
+            assert torch.equal(clean[n], got[n]), (n, bad)
+        assert (got["o"][blind] == 0).all() and (got["dq"][blind] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", [(3, 2, 2, 1, 300, 64), (3, 4, 2, 70, 130, 64), (24, 12, 12, 130, 150, 64), (3, 2, 1, 300, 40, 128)])
+def test_keys_that_nobody_sees_receive_nothing(ops, dtype, B, H, Hk, Sq, Sk, D):  # noqa: F811
+    """A query or a gradient that is not a number belongs to the visible keys; the others' gradients are zeros all the same."""
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=14)
+    kw = masks("mask", B, Sk)
+    hidden = kw["key_mask"] == 0
+    for name in ("q", "do"):
+        for bad in (math.nan, math.inf):
+            x = {"q": q.clone(), "do": do.clone()}
+            x[name][:, Sq // 2, 3::D] = bad
+            got, _ = run(ops, x["q"], k, v, x["do"], H, Hk, **kw)
+            for n in ("dk", "dv"):
+                assert (got[n][hidden] == 0).all(), (n, name, bad)
+            if name == "do":
+                assert not torch.isfinite(got["dv"].reshape(B, Sk, Hk, D)[..., 3][~hidden]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Sq", [1, 40, 200])
+def test_minus_infinity_in_the_table_hides(ops, dtype, Sq):  # noqa: F811
+    """Distances whose bias is -inf, or the lowest number of bf16 and fp32: rows that are left with nothing are rows that see nothing, the others as if
+    those keys were masked."""
+    B, H, Sk, D = 2, 3, 300, 64
+    q, k, v, do = make(B, H, H, Sq, Sk, D, dtype, seed=1)
+    table = torch.randn(32, H, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
+    table[15] = table[31] = -math.inf  # the far distances of both sides
+    buckets = ops.relative_buckets(32, 128)
+    kw = dict(scale=0.125, q_start=350, rel_bias=(table, buckets), key_count=torch.tensor([300, 200], dtype=torch.int32, device="cuda"))
+    got, lse = run(ops, q, k, v, do, H, H, **kw)
+    val, tol = reference(q, k, v, do, H, H, dtype, **kw)
+    blind = torch.isinf(val["lse"][:, 0])
+    assert blind.any() and torch.equal(torch.isinf(lse), torch.isinf(val["lse"]))
+    zero = {n: torch.nan_to_num(val[n]) for n in val}
+    # the element-wise bound holds the largest |score|, infinite here; instead: probabilities, score gradients and results rounded once each, of o and dq
+    # of size 1 (|v|, |k| of a few against probabilities that sum to 1), and fp32's rest of 300 terms
+    for n in ("o", "dq"):
+        assert (got[n][blind] == 0).all() and torch.isfinite(got[n]).all(), n
+        assert (got[n].double() - zero[n]).abs().max() <= 8 * U[dtype] * (1 + zero[n].abs().max()) + 300 * 2.0 ** -22, n
+    assert all(torch.isfinite(got[n]).all() for n in got)
+    if dtype != "fp16":  # fp16's lowest is an ordinary number to the scores
+        table[15] = table[31] = torch.finfo(DT[dtype]).min
+        low, low_lse = run(ops, q, k, v, do, H, H, **kw)
+        assert torch.equal(lse, low_lse) and all(torch.equal(got[n], low[n]) for n in got)
