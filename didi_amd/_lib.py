@@ -24,6 +24,7 @@ DT_BF16, DT_FP16, DT_FP32 = 0, 1, 2
 ACT_NONE, ACT_GELU, ACT_TANH, ACT_RELU, ACT_GELU_NEW = 0, 1, 2, 3, 4
 STEP_NONE, STEP_INIT, STEP_DDPM, STEP_EULER = 0, 1, 2, 3
 ERR_FAULT = -5
+ERR_OVERLAP = -6
 FAULT_LN_EXCHANGE, FAULT_FP16_RANGE = 1, 2
 ABI_VERSION = 7
 # didi_set_option keys (tuning switches for A/B runs; defaults = production path)

@@ -443,6 +443,7 @@ extern "C" const char* didi_error_string(int code) {
         case DIDI_ERR_UNSUPPORTED: return "shape not supported by the gfx950 kernels";
         case DIDI_ERR_LAUNCH: return "kernel launch failed";
         case DIDI_ERR_WORKSPACE: return "workspace too small";
+        case DIDI_ERR_OVERLAP: return "a result lies over an operand or another result";
         case DIDI_ERR_FAULT: return "device-side fault word is set (didi_fault_string names the bits)";
         default: return "unknown error";
     }

@@ -1,5 +1,8 @@
 // Host side of the attention of any lengths -- argument checks, how launches are cut, workspaces, the C entries -- and the dense relative
 // position bias with its gradient.  The mathematics and the kernels: long_attention.hpp.
+#include <numeric>
+#include <utility>
+
 #include "long_attention.hpp"
 
 using namespace la;
@@ -322,6 +325,91 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
     return DIDI_OK;
 }
 
+// An array of B dialogs of S rows in bytes; a contiguous one is a single row
+struct Span {
+    uintptr_t at;
+    int64_t n[2], step[2], w;  // outer and inner count and stride
+    Span(const void* p, int64_t B, int64_t batch, int64_t S, int64_t ld, int64_t width, int elem) : at(reinterpret_cast<uintptr_t>(p)), w(width * elem) {
+        n[0] = B; step[0] = batch * elem;
+        n[1] = S; step[1] = ld * elem;
+        if (!p || B == 0 || S == 0 || width == 0) n[0] = 0;
+        for (int k = 0; k < 2; ++k)
+            if (n[k] == 1) step[k] = 0;  // an only row's or dialog's stride does not count
+        if (n[0] > 1 && step[0] < step[1]) *this = turned();
+    }
+    Span turned() const {
+        Span s = *this;
+        std::swap(s.n[0], s.n[1]);
+        std::swap(s.step[0], s.step[1]);
+        return s;
+    }
+    Span(const void* p, int64_t bytes) : Span(p, 1, 0, 1, 0, bytes, 1) {}
+    bool empty() const { return n[0] == 0 || n[1] == 0; }
+    int64_t inner() const { return (n[1] - 1) * step[1] + w; }  // bytes from the first to behind the last of one outer step
+    int64_t all() const { return (n[0] - 1) * step[0] + inner(); }
+};
+
+// whether [0, a) and [d, d + b) share nothing when both repeat every g
+bool apart(int64_t d, int64_t a, int64_t b, int64_t g) {
+    if (g == 0) return false;
+    d = (d % g + g) % g;
+    return d >= a && d + b <= g;
+}
+
+// Two arrays are apart within a common stride of all rows, or of the outer steps, or the outer strides are one and the outer steps that meet have rows
+// that are
+bool steps_apart(const Span& a, const Span& b) {
+    const int64_t d = (int64_t)(b.at - a.at);
+    const int64_t outer = std::gcd(a.step[0], b.step[0]), inner = std::gcd(a.step[1], b.step[1]);
+    if (apart(d, a.w, b.w, std::gcd(outer, inner)) || apart(d, a.inner(), b.inner(), outer)) return true;
+    const int64_t P = std::max(a.step[0], b.step[0]);
+    if ((a.step[0] && a.step[0] != P) || (b.step[0] && b.step[0] != P) || P == 0 || a.inner() > P || b.inner() > P) return false;
+    const int64_t r = (d % P + P) % P;  // an outer step of a meets the one of b that begins r behind it and the one that begins P - r before it
+    for (const int64_t x : {r, r - P})
+        if (x < a.inner() && -x < b.inner() && !apart(x, a.w, b.w, inner)) return false;
+    return true;
+}
+
+// Whether two arrays share no element; false also where that cannot be shown.  An array of one row (dialog) a dialog (in all) is taken either way.
+bool disjoint(const Span& a, const Span& b) {
+    if (a.empty() || b.empty()) return true;
+    const int64_t d = (int64_t)(b.at - a.at);
+    if (d >= a.all() || -d >= b.all()) return true;
+    const bool ta = a.n[0] == 1 || a.n[1] == 1, tb = b.n[0] == 1 || b.n[1] == 1;
+    return steps_apart(a, b) || (ta && steps_apart(a.turned(), b)) || (tb && steps_apart(a, b.turned())) || (ta && tb && steps_apart(a.turned(), b.turned()));
+}
+
+// results over operands or over each other
+int check_overlap(const didi_long_attn_args* a, bool bwd, size_t workspace) {
+    const int e = a->dtype == DIDI_DT_FP32 ? 4 : 2;
+    const int64_t wq = (int64_t)a->heads * a->D, wk = (int64_t)a->kv_heads * a->D;
+    const int64_t table = a->table ? (int64_t)a->num_buckets * a->heads * e : 0;
+    const Span O(a->O, a->B, a->o_batch, a->Sq, a->ldo, wq, e), lo(a->O_lo, a->B, a->o_batch, a->Sq, a->ldo, wq, e), lse(a->lse, (int64_t)a->B * a->heads * a->Sq * 4);
+    const Span ws(a->workspace, (int64_t)workspace);
+    const Span in[] = {Span(a->Q, a->B, a->q_batch, a->Sq, a->ldq, wq, e), Span(a->K, a->B, a->k_batch, a->Sk, a->ldk, wk, e),
+                       Span(a->V, a->B, a->v_batch, a->Sk, a->ldv, wk, e), Span(a->key_mask, (int64_t)a->B * a->Sk * 4), Span(a->key_count, (int64_t)a->B * 4),
+                       Span(a->table, table), Span(a->buckets, a->table ? (2 * (int64_t)a->max_distance + 1) * 4 : 0)};
+    auto clear_of = [&](const Span& out) {
+        for (const Span& s : in)
+            if (!disjoint(out, s)) return false;
+        return true;
+    };
+    if (!bwd) {
+        const bool ok = clear_of(O) && clear_of(lo) && clear_of(lse) && clear_of(ws) && disjoint(O, lo) && disjoint(O, lse) && disjoint(O, ws) && disjoint(lo, lse) &&
+                        disjoint(lo, ws) && disjoint(lse, ws);
+        return ok ? DIDI_OK : DIDI_ERR_OVERLAP;
+    }
+    const Span out[] = {Span(a->dQ, a->B, a->dq_batch, a->Sq, a->lddq, wq, e), Span(a->dK, a->B, a->dk_batch, a->Sk, a->lddk, wk, e),
+                        Span(a->dV, a->B, a->dv_batch, a->Sk, a->lddv, wk, e), Span(a->dtable, table), ws};
+    const Span dO(a->dO, a->B, a->do_batch, a->Sq, a->lddo, wq, e);
+    for (const Span& x : out) {
+        if (!clear_of(x) || !disjoint(x, O) || !disjoint(x, lo) || !disjoint(x, lse) || !disjoint(x, dO)) return DIDI_ERR_OVERLAP;
+        for (const Span* y = out; y != &x; ++y)
+            if (!disjoint(x, *y)) return DIDI_ERR_OVERLAP;
+    }
+    return DIDI_OK;
+}
+
 LaParams make_params(const didi_long_attn_args* a, bool bwd) {
     LaParams p{};
     p.B = a->B; p.H = a->heads; p.Hk = a->kv_heads; p.G = a->heads / a->kv_heads; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D;
@@ -364,6 +452,7 @@ extern "C" int didi_long_attention_forward(const didi_long_attn_args* a, void* s
     const Plan q = make_plan(a);
     if (q.fwd_bytes && (!a->workspace || a->workspace_bytes < q.fwd_bytes)) return DIDI_ERR_WORKSPACE;
     DIDI_CHECK_ARG((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0);
+    if (const int rc = check_overlap(a, false, q.fwd_bytes)) return rc;
     LaParams p = make_params(a, false);
     set_cut(p, q.f);
     p.part = static_cast<float*>(a->workspace);
@@ -378,6 +467,7 @@ extern "C" int didi_long_attention_backward(const didi_long_attn_args* a, void* 
     const Plan q = make_plan(a);
     if (q.bwd_bytes && (!a->workspace || a->workspace_bytes < q.bwd_bytes)) return DIDI_ERR_WORKSPACE;
     DIDI_CHECK_ARG((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0);
+    if (const int rc = check_overlap(a, true, q.bwd_bytes)) return rc;
     LaParams p = make_params(a, true);
     char* ws = static_cast<char*>(a->workspace);
     p.rows = reinterpret_cast<float*>(ws);

@@ -775,7 +775,10 @@ def _long_run(dev, what, fn, backward, fields):
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.check(_launch(dev, fn, a), what)
+    rc = _launch(dev, fn, a)
+    if rc == _lib.ERR_OVERLAP:
+        raise ValueError("out may not lie over an operand or another result")
+    _lib.check(rc, what)
 
 
 def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_mask=None, key_count=None, scale=None, rel_bias=None, drop_p=0.0,
@@ -788,13 +791,11 @@ def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_
     gives zeros, and what lies at keys that no row of a dialog sees is never used.  ``scale``: default 1/sqrt(D).  ``rel_bias`` = (table [num_buckets, heads],
     relative_buckets(...)): a learned bias by the distance from query q_start + i to the key, added to the scaled scores.  ``drop_p``,
     ``seed``, ``offset``: dropout of the probabilities, ``attention_train``'s mask.
-    ``need_grad``: -> (o, saved) for ``cross_attention_backward``.  ``out``: written to (a view as for q, not over an operand)."""
+    ``need_grad``: -> (o, saved) for ``cross_attention_backward``.  ``out``: written to (a view as for q; it may share a buffer with operands, but no element)."""
     before, after = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
     dev, shape = q.device, q.shape
     o = torch.empty(shape, dtype=q.dtype, device=dev) if out is None else out
     O, ob, ldo = _rows("out", o, shape, q.dtype, dev)
-    if O and O in before[12:15]:
-        raise ValueError("out may not lie over an operand")
     saved, lse, lo = None, 0, 0
     if need_grad:
         # the output's remainder plane: D = do . o enters every score gradient, and the bias gradient's sums of those cancel; from o's own 8 or 11
@@ -809,8 +810,8 @@ def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_
 def cross_attention_backward(q, k, v, o, saved, dO, heads, kv_heads=None, causal=False, q_start=0, key_mask=None, key_count=None, scale=None,
                              rel_bias=None, drop_p=0.0, seed=0, offset=0, out=None):
     """Backward of ``cross_attention(..., need_grad=True)`` with the same arguments -> (dq, dk, dv), and dtable where a bias was given.
-    ``out`` = (dq, dk, dv): views to write into (e.g. the thirds of a fused projection's gradient), not over operands; default fresh
-    contiguous tensors.  fp16: gradients beyond the type's range are infinite, as a loss scaler expects.
+    ``out`` = (dq, dk, dv): views to write into (e.g. the thirds of a fused projection's gradient) that share no element with operands or each
+    other; default fresh contiguous tensors.  fp16: gradients beyond the type's range are infinite, as a loss scaler expects.
     Deterministic."""
     before, after = _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, scale, rel_bias, drop_p, seed, offset)
     dev, dt, shape, kv_shape = q.device, q.dtype, q.shape, k.shape
@@ -828,8 +829,6 @@ def cross_attention_backward(q, k, v, o, saved, dO, heads, kv_heads=None, causal
     dq, dqb, lddq = _rows("dq", grads[0], shape, dt, dev)
     dk, dkb, lddk = _rows("dk", grads[1], kv_shape, dt, dev)
     dv, dvb, lddv = _rows("dv", grads[2], kv_shape, dt, dev)
-    if out is not None and ({dq, dk, dv} & {O, G, *before[12:15]}) - {0}:
-        raise ValueError("out may not lie over an operand")
     dtable = 0
     if rel_bias is not None:
         grads += (torch.empty_like(rel_bias[0]),)

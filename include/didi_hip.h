@@ -42,6 +42,7 @@ enum {
     DIDI_ERR_UNSUPPORTED = -2, /* shape outside what the kernels are built for */
     DIDI_ERR_LAUNCH = -3,      /* hipLaunchKernel reported an error */
     DIDI_ERR_WORKSPACE = -4,   /* workspace too small */
+    DIDI_ERR_OVERLAP = -6,     /* a result would lie over an operand or another result */
     DIDI_ERR_FAULT = -5        /* didi_fault_read: the device-side fault word is non-zero (bits: DIDI_FAULT_*) */
 };
 
@@ -704,7 +705,8 @@ int didi_train_target_backward(const float* x0hat, const float* emb, const float
  * O_lo (BF16 / FP16, optional): the output's remainder plane; the backward adds it to O where it is given: every score gradient holds D = do . o.
  * Strides in elements: ld* between rows, *_batch between dialogs (inputs may repeat a dialog with 0).
  * 16-byte aligned bases and strides.  D % 8 == 0 (FP32: % 4), D <= 128; max_distance <= 512, num_buckets <= 1024.
- * Any of B, Sq, Sk may be 0.  Neither call has atomics whose order could change a result.
+ * Results may share a buffer with operands and with each other (the thirds of a fused projection), but no element: DIDI_ERR_OVERLAP otherwise, and
+ * where rows of different strides are interleaved so that it cannot be told.  Any of B, Sq, Sk may be 0.  Neither call has atomics whose order could change a result.
  * workspace: didi_long_attention_workspace_bytes(args, backward) bytes, 16-byte aligned, NULL where that is 0.  Its size depends on the shape
  * fields, table, dtable and dtype alone. */
 enum { DIDI_DT_BF16 = 0, DIDI_DT_FP16 = 1, DIDI_DT_FP32 = 2 };

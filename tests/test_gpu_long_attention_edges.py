@@ -296,3 +296,45 @@ def test_minus_infinity_in_the_table_hides(ops, dtype, Sq):  # noqa: F811
         table[15] = table[31] = torch.finfo(DT[dtype]).min
         low, low_lse = run(ops, q, k, v, do, H, H, **kw)
         assert torch.equal(lse, low_lse) and all(torch.equal(got[n], low[n]) for n in got)
+
+
+def test_results_that_share_elements_are_refused(ops):  # noqa: F811
+    B, S, H, D = 2, 40, 2, 32
+    W = H * D
+    buf = torch.randn(B, S, 4 * W, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    q, k, v = buf[:, :, :W], buf[:, :, W:2 * W], buf[:, :, 2 * W:3 * W]
+    do = torch.randn(B, S, W, device="cuda").bfloat16()
+    flat = buf.view(-1)
+    for out in (buf[:, :, W - 8:2 * W - 8], buf[:, :, 2 * W + 8:3 * W + 8], flat[W // 2:][:B * S * W].view(B, S, W), k, buf[:, :, 3 * W - 8:4 * W - 8], q):
+        with pytest.raises(ValueError, match="operand"):
+            ops.cross_attention(q, k, v, H, out=out)
+    o, saved = ops.cross_attention(q, k, v, H, need_grad=True)
+    a, b, c = (torch.empty_like(do) for _ in range(3))
+    two = torch.empty(B, S, 2 * W, dtype=do.dtype, device="cuda")
+    for out in ((a, b, b), (a, a, c), (a, b, a), (a, two[:, :, :W], two[:, :, W - 8:2 * W - 8]), (buf[:, :, W // 2:W + W // 2], b, c), (a, saved[1], c), (o, b, c), (a, do, c)):
+        with pytest.raises(ValueError, match="operand"):
+            ops.cross_attention_backward(q, k, v, o, saved, do, H, out=out)
+
+
+def test_results_between_the_operands_are_written(ops):  # noqa: F811
+    """Columns, rows, dialogs and ranges of the operands' own buffer that hold none of their elements."""
+    B, S, H, D = 3, 35, 2, 32
+    W = H * D
+    g = torch.Generator().manual_seed(4)
+    plain = [torch.randn(B, S, W, generator=g).bfloat16().cuda() for _ in range(4)]
+    want, saved = ops.cross_attention(*plain[:3], H, need_grad=True)
+    grads = ops.cross_attention_backward(*plain[:3], want, saved, plain[3], H)
+    layouts = [lambda t, n: t.view(B, S, 8, W)[:, :, n],  # columns of a fused projection
+               lambda t, n: t.view(B, 8, S, W)[:, n],  # ranges of a dialog's buffer
+               lambda t, n: t.view(8, B, S, W)[n],
+               lambda t, n: t.as_strided((B, S, W), ((8 * S + 1) * W, 8 * W, 1), n * W)]  # every eighth row, dialogs an odd number of rows apart
+    for at in layouts:
+        buf = torch.zeros(8 * B * S * W + B * W, dtype=torch.bfloat16, device="cuda")
+        view = [at(buf if at is layouts[-1] else buf[:8 * B * S * W], n) for n in range(8)]
+        for x, y in zip(view, plain):
+            x.copy_(y)
+        o, saved = ops.cross_attention(*view[:3], H, need_grad=True, out=view[4])
+        assert torch.equal(o, want)
+        got = ops.cross_attention_backward(*view[:3], o, saved, view[3], H, out=view[5:8])
+        assert all(torch.equal(x, y) for x, y in zip(got, grads))
+        assert all(torch.equal(x, y) for x, y in zip(view, plain))  # the operands are as they were
