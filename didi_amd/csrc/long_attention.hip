@@ -319,7 +319,8 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
         if (!o.p) continue;
         DIDI_CHECK_ARG(o.ld >= o.w || o.S == 1);
         DIDI_CHECK_ARG(o.batch >= 0 && aligned(o.p, o.batch, o.ld, 16, e));
-        if (o.written && a->B > 1) DIDI_CHECK_ARG(o.batch >= (int64_t)(o.S - 1) * o.ld + o.w);  // dialogs of an output may not overlap
+        // dialogs of an output may not overlap: one behind the other, or row by row in turn
+        if (o.written && a->B > 1) DIDI_CHECK_ARG(o.batch >= (int64_t)(o.S - 1) * o.ld + o.w || (o.batch >= o.w && o.ld >= (int64_t)(a->B - 1) * o.batch + o.w));
     }
     DIDI_CHECK_ARG(!bwd || a->lse || a->B == 0 || a->Sq == 0);
     return DIDI_OK;

@@ -305,7 +305,8 @@ def test_results_that_share_elements_are_refused(ops):  # noqa: F811
     q, k, v = buf[:, :, :W], buf[:, :, W:2 * W], buf[:, :, 2 * W:3 * W]
     do = torch.randn(B, S, W, device="cuda").bfloat16()
     flat = buf.view(-1)
-    for out in (buf[:, :, W - 8:2 * W - 8], buf[:, :, 2 * W + 8:3 * W + 8], flat[W // 2:][:B * S * W].view(B, S, W), k, buf[:, :, 3 * W - 8:4 * W - 8], q):
+    for out in (buf[:, :, W - 8:2 * W - 8], buf[:, :, 2 * W + 8:3 * W + 8], flat[W // 2:][:B * S * W].view(B, S, W), k, buf[:, :, 3 * W - 8:4 * W - 8], q,
+                flat.as_strided((B, S, W), (W, B * W, 1))):
         with pytest.raises(ValueError, match="operand"):
             ops.cross_attention(q, k, v, H, out=out)
     o, saved = ops.cross_attention(q, k, v, H, need_grad=True)
@@ -327,6 +328,8 @@ def test_results_between_the_operands_are_written(ops):  # noqa: F811
     layouts = [lambda t, n: t.view(B, S, 8, W)[:, :, n],  # columns of a fused projection
                lambda t, n: t.view(B, 8, S, W)[:, n],  # ranges of a dialog's buffer
                lambda t, n: t.view(8, B, S, W)[n],
+               lambda t, n: t.view(S, B, 8, W)[:, :, n].transpose(0, 1),  # rows of the dialogs in turn
+               lambda t, n: t.view(8, S, B, W)[n].transpose(0, 1),
                lambda t, n: t.as_strided((B, S, W), ((8 * S + 1) * W, 8 * W, 1), n * W)]  # every eighth row, dialogs an odd number of rows apart
     for at in layouts:
         buf = torch.zeros(8 * B * S * W + B * W, dtype=torch.bfloat16, device="cuda")

@@ -18,6 +18,7 @@ APART = dict(Q=MB, K=2 * MB, V=3 * MB, O=4 * MB, O_lo=5 * MB, lse=6 * MB, dO=7 *
     # a column of the neighbour's third, rows that meet another dialog's, the other order of dialogs and rows
     dict(Q=MB, ldq=3 * W, q_batch=30 * W, O=MB + 2 * W - 16, ldo=3 * W, o_batch=30 * W),
     dict(Q=MB, ldq=W, q_batch=11 * W, O=MB + 2 * 2 * W, ldo=W, o_batch=11 * W),
+    dict(Q=MB, ldq=2 * W, q_batch=W, O=MB + 2 * 4 * W, ldo=2 * W, o_batch=W),
     dict(Q=MB, ldq=2 * W, q_batch=W, O=MB + 2 * 3 * W, ldo=W, o_batch=10 * W)])
 def test_forward_refuses_results_over_operands(kw):
     assert lib.didi_long_attention_forward(args(**{**APART, **kw}), None) == OVERLAP
@@ -33,3 +34,8 @@ def test_backward_refuses_results_over_operands_and_each_other(kw):
 
 def test_the_refusal_has_a_text():
     assert b"operand" in lib.didi_error_string(OVERLAP)
+
+
+@pytest.mark.parametrize("kw", [dict(o_batch=W - 8, ldo=2 * W), dict(o_batch=W, ldo=2 * W - 8), dict(o_batch=0, ldo=2 * W), dict(o_batch=10 * W - 8, ldo=W)])
+def test_dialogs_of_a_result_over_each_other_are_refused(kw):
+    assert lib.didi_long_attention_forward(args(**{**APART, **kw}), None) == -1
