@@ -297,6 +297,7 @@ int check_args(const didi_long_attn_args* a, bool bwd) {
     const int64_t lim = (int64_t)1 << 30;
     for (int ld : {a->ldq, a->ldk, a->ldv, a->lddo})  // a tile of up to 128 rows lies within 2 GiB
         if (ld > (1 << 21)) return DIDI_ERR_UNSUPPORTED;
+    if ((int64_t)a->heads * a->D > (1 << 21)) return DIDI_ERR_UNSUPPORTED;
     if ((int64_t)a->Sq * a->heads > lim || cdiv((int64_t)a->Sq * a->heads, 32) > 65535 || cdiv(a->Sk, 32) > 65535 || a->Sk > lim || (int64_t)a->q_start + a->Sq > lim || (int64_t)a->B * a->heads > (1 << 20)) return DIDI_ERR_UNSUPPORTED;
     const int64_t wq = (int64_t)a->heads * a->D, wk = (int64_t)a->kv_heads * a->D;
     const int e = f32 ? 4 : 2;
@@ -425,7 +426,10 @@ LaParams make_params(const didi_long_attn_args* a, bool bwd) {
     p.dQ = a->dQ; p.dK = a->dK; p.dV = a->dV;
     p.qb = a->q_batch; p.kb = a->k_batch; p.vb = a->v_batch; p.ob = a->o_batch; p.dob = a->do_batch;
     p.dqb = a->dq_batch; p.dkb = a->dk_batch; p.dvb = a->dv_batch;
-    p.ldq = a->ldq; p.ldk = a->ldk; p.ldv = a->ldv; p.ldo = a->ldo; p.lddo = a->lddo; p.lddq = a->lddq; p.lddk = a->lddk; p.lddv = a->lddv;
+    // an only row's stride does not count, but the kernels' tiles are cut at rows x stride
+    auto ld = [a](int stride, int S, int heads) { return S == 1 ? heads * a->D : stride; };
+    p.ldq = ld(a->ldq, a->Sq, a->heads); p.ldo = ld(a->ldo, a->Sq, a->heads); p.lddo = ld(a->lddo, a->Sq, a->heads); p.lddq = ld(a->lddq, a->Sq, a->heads);
+    p.ldk = ld(a->ldk, a->Sk, a->kv_heads); p.ldv = ld(a->ldv, a->Sk, a->kv_heads); p.lddk = ld(a->lddk, a->Sk, a->kv_heads); p.lddv = ld(a->lddv, a->Sk, a->kv_heads);
     p.lse = a->lse;
     p.table = a->table; p.map = a->buckets; p.nb = a->num_buckets; p.maxd = a->table ? a->max_distance : 0;
     p.thr = (uint32_t)fminf(a->drop_p * 4294967296.0f, 4294967040.0f);

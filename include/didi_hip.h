@@ -703,7 +703,7 @@ int didi_train_target_backward(const float* x0hat, const float* emb, const float
  * dtype BF16 / FP16: one product per pair, probabilities and score gradients rounded to that type; FP32: fp32 products throughout.
  * FP16 score gradients are scaled by powers of two so that none overflows on the way; a result beyond the type's range is infinite.
  * O_lo (BF16 / FP16, optional): the output's remainder plane; the backward adds it to O where it is given: every score gradient holds D = do . o.
- * Strides in elements: ld* between rows, *_batch between dialogs (inputs may repeat a dialog with 0).
+ * Strides in elements: ld* between rows (of an only row: any multiple of 16 bytes), *_batch between dialogs (inputs may repeat a dialog with 0).
  * 16-byte aligned bases and strides.  D % 8 == 0 (FP32: % 4), D <= 128; max_distance <= 512, num_buckets <= 1024.
  * Results may share a buffer with operands and with each other (the thirds of a fused projection), but no element: DIDI_ERR_OVERLAP otherwise, and
  * where rows of different strides are interleaved so that it cannot be told.  Any of B, Sq, Sk may be 0.  Neither call has atomics whose order could change a result.

@@ -341,3 +341,34 @@ def test_results_between_the_operands_are_written(ops):  # noqa: F811
         got = ops.cross_attention_backward(*view[:3], o, saved, view[3], H, out=view[5:8])
         assert all(torch.equal(x, y) for x, y in zip(got, grads))
         assert all(torch.equal(x, y) for x, y in zip(view, plain))  # the operands are as they were
+
+
+@pytest.mark.parametrize("ld", [0, 8, -64, 4096])
+@pytest.mark.parametrize("Sq,Sk", [(1, 1), (1, 70), (70, 1)])
+def test_the_row_stride_of_an_only_row_does_not_count(ops, Sq, Sk, ld):  # noqa: F811
+    """C callers: an operand of one row with any row stride."""
+    import ctypes as C
+
+    from didi_amd import _lib
+
+    B, H, Hk, D = 2, 4, 2, 64
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, "bf16", seed=3)
+    o, saved = ops.cross_attention(q, k, v, H, kv_heads=Hk, need_grad=True)
+    want = (o, *ops.cross_attention_backward(q, k, v, o, saved, do, H, kv_heads=Hk))
+    W, WK = H * D, Hk * D
+    lq, lk = ld if Sq == 1 else W, ld if Sk == 1 else WK
+    got = [torch.zeros_like(x) for x in want]
+    lse, lo = torch.empty_like(saved[0]), torch.empty_like(o)
+    a = _lib.LongAttnArgs(B, H, Hk, Sq, Sk, D, _lib.DT_BF16, 0, 0, 0.0)
+    for name, x in dict(Q=q, K=k, V=v, O=got[0], O_lo=lo, lse=lse, dO=do, dQ=got[1], dK=got[2], dV=got[3]).items():
+        setattr(a, name, x.data_ptr())
+    a.q_batch = a.o_batch = a.do_batch = a.dq_batch = Sq * W
+    a.k_batch = a.v_batch = a.dk_batch = a.dv_batch = Sk * WK
+    a.ldq = a.ldo = a.lddo = a.lddq = lq
+    a.ldk = a.ldv = a.lddk = a.lddv = lk
+    ws = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+    assert max(_lib.lib.didi_long_attention_workspace_bytes(C.byref(a), n) for n in (0, 1)) <= ws.numel()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _lib.check(_lib.lib.didi_long_attention_forward(C.byref(a), _lib.current_stream()))
+    _lib.check(_lib.lib.didi_long_attention_backward(C.byref(a), _lib.current_stream()))
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(lse, saved[0])

@@ -39,3 +39,8 @@ def test_the_refusal_has_a_text():
 @pytest.mark.parametrize("kw", [dict(o_batch=W - 8, ldo=2 * W), dict(o_batch=W, ldo=2 * W - 8), dict(o_batch=0, ldo=2 * W), dict(o_batch=10 * W - 8, ldo=W)])
 def test_dialogs_of_a_result_over_each_other_are_refused(kw):
     assert lib.didi_long_attention_forward(args(**{**APART, **kw}), None) == -1
+
+
+def test_rows_too_wide_for_a_tile_are_refused():
+    wide = dict(heads=1 << 16, kv_heads=1 << 16, Sq=1, Sk=1, D=64, B=1, ldq=0, ldk=0, ldv=0, ldo=0)
+    assert lib.didi_long_attention_forward(args(**{**APART, **wide}), None) == -2
