@@ -284,7 +284,7 @@ bool aligned(const void* p, int64_t batch, int64_t ld, int bytes, int elem) {
 int check_args(const didi_long_attn_args* a, bool bwd) {
     DIDI_CHECK_ARG(a && a->B >= 0 && a->Sq >= 0 && a->Sk >= 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->D > 0);
     DIDI_CHECK_ARG(a->dtype == DIDI_DT_BF16 || a->dtype == DIDI_DT_FP16 || a->dtype == DIDI_DT_FP32);
-    DIDI_CHECK_ARG(a->scale >= 0.f && a->scale < INFINITY && a->drop_p >= 0.f && a->drop_p < 1.f && a->q_start >= 0);
+    DIDI_CHECK_ARG((a->scale == 0.f || (a->scale >= 0x1p-126f && a->scale <= 0x1p127f)) && a->drop_p >= 0.f && a->drop_p < 1.f && a->q_start >= 0);
     const bool f32 = a->dtype == DIDI_DT_FP32;
     DIDI_CHECK_ARG(!(f32 && a->O_lo));
     if (a->D > 128 || a->D % (f32 ? 4 : 8) != 0) return DIDI_ERR_UNSUPPORTED;

@@ -740,8 +740,8 @@ def _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, s
         raise ValueError(f"heads={heads} must divide the width {HD} and be a multiple of kv_heads={kv_heads}")
     if scale is None:
         scale = 0.0
-    elif not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale={scale} must be positive and finite")
+    elif not 2.0 ** -126 <= scale <= 2.0 ** 127:  # a float for the kernels, times log2 e: 0 would mean the default
+        raise ValueError(f"scale={scale} must be positive and within fp32's normal range")
     D = HD // heads
     kv_shape = (B, Sk, kv_heads * D)
     Q, qb, ldq = _rows("q", q, shape, dt, dev)

@@ -714,7 +714,7 @@ typedef struct didi_long_attn_args {
     int B, heads, kv_heads, Sq, Sk, D;
     int dtype;
     int causal, q_start;       /* query i stands at position q_start + i (causal limit and distances) */
-    float scale;               /* 0 = 1/sqrt(D) */
+    float scale;               /* 0 = 1/sqrt(D); otherwise 2^-126 .. 2^127 */
     const int32_t* key_mask;   /* [B, Sk] or NULL */
     const int32_t* key_count;  /* [B] or NULL: keys from key_count[b] on are not visible */
     const void *Q, *K, *V;

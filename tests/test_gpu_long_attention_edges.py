@@ -372,3 +372,17 @@ def test_the_row_stride_of_an_only_row_does_not_count(ops, Sq, Sk, ld):  # noqa:
     _lib.check(_lib.lib.didi_long_attention_forward(C.byref(a), _lib.current_stream()))
     _lib.check(_lib.lib.didi_long_attention_backward(C.byref(a), _lib.current_stream()))
     assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(lse, saved[0])
+
+
+def test_the_ends_of_the_scale(ops):  # noqa: F811
+    """A scale that rounds to zero in fp32 meant the default."""
+    q, k, v, _ = make(1, 2, 2, 5, 9, 32, "fp32")
+    for scale in (1e-50, 1e-40, 0.0, -1.0, 3e38, 1e39, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            ops.cross_attention(q, k, v, 2, scale=scale)
+    o = ops.cross_attention(q, k, v, 2, scale=2.0 ** -126)  # scores of zero: the mean of the values
+    # a sum of nine terms, divided once: 12 roundings of fp32
+    assert ((o.double() - v.double().mean(1, keepdim=True)).abs() <= 12 * 2.0 ** -24 * v.double().abs().mean(1, keepdim=True)).all()
+    q.zero_()
+    top = ops.cross_attention(q, k, v, 2, scale=2.0 ** 127)
+    assert ((top.double() - v.double().mean(1, keepdim=True)).abs() <= 12 * 2.0 ** -24 * v.double().abs().mean(1, keepdim=True)).all()

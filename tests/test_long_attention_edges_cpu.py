@@ -44,3 +44,8 @@ def test_dialogs_of_a_result_over_each_other_are_refused(kw):
 def test_rows_too_wide_for_a_tile_are_refused():
     wide = dict(heads=1 << 16, kv_heads=1 << 16, Sq=1, Sk=1, D=64, B=1, ldq=0, ldk=0, ldv=0, ldo=0)
     assert lib.didi_long_attention_forward(args(**{**APART, **wide}), None) == -2
+
+
+@pytest.mark.parametrize("scale", [1e-40, 2.0 ** -149, 3e38, -1.0, float("nan")])
+def test_a_scale_that_fp32_cannot_hold_is_refused(scale):
+    assert lib.didi_long_attention_forward(args(**{**APART, "scale": scale}), None) == -1
