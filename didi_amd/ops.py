@@ -765,6 +765,8 @@ def _long_args(q, k, v, heads, kv_heads, causal, q_start, key_mask, key_count, s
         raise ValueError(f"drop_p={drop_p} must be in [0, 1)")
     if not drop_p:
         seed = offset = 0
+    else:  # 64 bits of each, as attention_train takes them
+        seed, offset = int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF
     before = (B, heads, kv_heads, Sq, Sk, D, code, 1 if causal else 0, q_start, scale, mask, count, Q, K, V, qb, kb, vb, ldq, ldk, ldv)
     return before, (table, buckets, nb, maxd, drop_p, seed, offset)
 

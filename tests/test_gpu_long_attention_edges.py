@@ -386,3 +386,14 @@ def test_the_ends_of_the_scale(ops):  # noqa: F811
     q.zero_()
     top = ops.cross_attention(q, k, v, 2, scale=2.0 ** 127)
     assert ((top.double() - v.double().mean(1, keepdim=True)).abs() <= 12 * 2.0 ** -24 * v.double().abs().mean(1, keepdim=True)).all()
+
+
+@pytest.mark.parametrize("seed,offset", [(-5, 0), (2 ** 64 - 5, 3), (7, -(2 ** 40)), (2 ** 64 + 3, 2 ** 64 - 1), (torch.tensor(11), torch.tensor(1 << 34))])
+def test_seeds_are_taken_as_the_training_attention_takes_them(ops, seed, offset):  # noqa: F811
+    B, H, S, D = 2, 2, 20, 32
+    q, k, v, _ = make(B, H, H, S, S, D, "fp32", seed=15)
+    v.copy_((torch.arange(S * H * D).reshape(S, H * D) % S == torch.arange(S)[:, None]).float().cuda()[None])  # ones and zeros: o sums probabilities
+    kw = dict(drop_p=0.5, seed=seed, offset=offset)
+    a, b = ops.cross_attention(q, k, v, H, **kw), ops.attention_train(q, k, v, H, **kw)
+    # probabilities to fp32's 32 + 8 roundings of scores of size 8 in both; another mask would differ by a probability, 0.05
+    assert (a - b).abs().max() < 1e-4 and (a != ops.cross_attention(q, k, v, H)).any()
