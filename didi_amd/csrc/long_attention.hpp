@@ -3,6 +3,7 @@
 // padding, key masks, a causal limit, keys shared by groups of heads, a learned relative position bias by buckets, and dropout.
 //
 //   visible(b, i, j) = j < count[b] and mask[b, j] != 0 and (not causal or j <= q_start + i)
+//   (count[b] < 0: mask and scores do not count in that dialog, t = 0 at all keys that causal leaves: what additive masks of the lowest value come to)
 //   t_ij  = scale q_i . k_j + table[bucket(j - q_start - i)][head]          p_ij = exp(t_ij - lse_i) over the visible j, 0 elsewhere
 //   o_i   = sum_j drop(p_ij) v_j           lse_i = log sum_j exp(t_ij)
 //   ds_ij = p_ij (drop(do_i . v_j) - do_i . o_i)
@@ -354,10 +355,13 @@ __device__ __forceinline__ float max_halves(float x) {
 // a packed row's head within the group, and its query
 __device__ __forceinline__ int row_group(const LaParams& p, int r) { return p.Gr > 1 ? (int)((unsigned)r / (unsigned)p.Sq) : 0; }
 
-__device__ __forceinline__ int visible_end(const LaParams& p, int b) {
-    int e = p.Sk;
-    if (p.count) e = min(e, max(0, __builtin_amdgcn_readfirstlane(p.count[b])));
-    return e;
+// keys of a dialog; `even`: its count is negative, every key weighs the same
+__device__ __forceinline__ int visible_end(const LaParams& p, int b, bool& even) {
+    even = false;
+    if (!p.count) return p.Sk;
+    const int n = __builtin_amdgcn_readfirstlane(p.count[b]);
+    even = n < 0;
+    return even ? p.Sk : min(n, p.Sk);
 }
 
 // Which keys of a dialog a workgroup's rows may see, 64 a word: the key mask is turned into bits ahead of the tiles, 64 words at a time into a
@@ -376,8 +380,8 @@ struct Keys {
             if (lane == 0) ring[word & 127] = bits;
         }
     }
-    __device__ __forceinline__ void start(const LaParams& p, int b, int end_, uint64_t* ring_, int key0, int tid) {
-        row = p.mask && end_ > 0 ? p.mask + (int64_t)b * p.Sk : nullptr;
+    __device__ __forceinline__ void start(const LaParams& p, int b, bool even, int end_, uint64_t* ring_, int key0, int tid) {
+        row = p.mask && end_ > 0 && !even ? p.mask + (int64_t)b * p.Sk : nullptr;
         ring = ring_;
         end = end_;
         window = key0 >> 12;
@@ -430,6 +434,7 @@ template <class T>
 struct Bias {
     int t[2];
     float f[2];
+    bool even = false;  // no bias at all
     __device__ __forceinline__ void ask(const LaParams& p, int x0, int tid) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) t[k] = p.map[min(max(x0 + tid + 256 * k - PADB, 0), 2 * p.maxd)];
@@ -442,7 +447,7 @@ struct Bias {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int x = x0 + tid + 256 * k;
-            if (x < 2 * p.maxd + 1 + 2 * PADB) v[x] = t[k] >= 0 && t[k] < p.nb ? f[k] * LOG2E : __builtin_nanf("");
+            if (x < 2 * p.maxd + 1 + 2 * PADB) v[x] = even ? 0.f : t[k] >= 0 && t[k] < p.nb ? f[k] * LOG2E : __builtin_nanf("");
         }
     }
     // stores what was asked for and the rest; [lo, hi]: outside these distances the buckets are those of the ends (sh: 8 ints)
@@ -480,9 +485,10 @@ struct Bias {
     }
 };
 template <class T>
-__device__ __forceinline__ void bias_fill(const LaParams& p, int head, float* v, int tid) {
+__device__ __forceinline__ void bias_fill(const LaParams& p, int head, bool even, float* v, int tid) {
     for (int x0 = 0; x0 < 2 * p.maxd + 1 + 2 * PADB; x0 += 512) {
         Bias<T> b;
+        b.even = even;
         b.ask(p, x0, tid);
         b.gather(p, head);
         b.store(p, v, x0, tid);
@@ -540,7 +546,8 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     const int rt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.HG), hg = (int)blockIdx.x - b * p.HG;
     const int head0 = p.Gr > 1 ? hg * p.Gr : hg, kvh = p.Gr > 1 ? hg : p.G > 1 ? hg / p.G : hg;
     const int R = p.Gr * p.Sq, rbase = rt * C::ROWS, wr = wave / WK, wk = wave % WK, rw = rbase + wr * 32;
-    int kend = visible_end(p, b);
+    bool even;
+    int kend = visible_end(p, b, even);
     if (p.causal) {
         const int last = min(R, rbase + C::ROWS) - 1;
         const int g0 = row_group(p, rbase), g1 = row_group(p, last);
@@ -551,7 +558,10 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
 
     const int r = rw + (lane & 31), g = r < R ? row_group(p, r) : 0, i = r < R ? r - g * p.Sq : 0, head = head0 + g, pos = p.q_start + i;
     const int64_t rowid = ((int64_t)b * p.H + head) * p.Sq + i;
-    if constexpr (BIAS) bias.gather(p, head0);
+    if constexpr (BIAS) {
+        bias.even = even;
+        bias.gather(p, head0);
+    }
     Frag<T, DP> q;
     q.load(p.Q, (int64_t)b * p.qb + (int64_t)i * p.ldq + head * p.D, r < R, p.D, h);
     const int64_t kbase = (int64_t)b * p.kb + kvh * p.D, vbase = (int64_t)b * p.vb + kvh * p.D;
@@ -559,7 +569,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
     tk.init(p.ldk, p.D, tid);
     tv.init(p.ldv, p.D, tid);
     Keys keys;
-    keys.start(p, b, kend, ring, t0 * C::BN, tid);
+    keys.start(p, b, even, kend, ring, t0 * C::BN, tid);
     int slot = 0;  // where the next tile goes
     auto issue = [&](int t) {
         const uint32_t img = slot * 2 * C::IMG;
@@ -583,6 +593,7 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
     float m = -INFINITY, l = 0.f;  // maximum in units of t (base 2: with the bias) or of q . k; this lane's half of the row's sum
+    if (even) q.clear();
     q.settle();
     const float mul = BIAS ? 1.f : p.sc;
 
@@ -846,7 +857,8 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     const bool rok = r < R;
     const int g = rok ? row_group(p, r) : 0, i = rok ? r - g * p.Sq : 0, head = head0 + g, pos = p.q_start + i;
     const int64_t rowid = ((int64_t)b * p.H + head) * p.Sq + i;
-    int kend = visible_end(p, b);
+    bool even;
+    int kend = visible_end(p, b, even);
     if (p.causal) {
         const int last = min(R, rbase + C::ROWS) - 1;
         const int g0 = row_group(p, rbase), g1 = row_group(p, last);
@@ -855,7 +867,10 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     const int tiles = (kend + C::BN - 1) / C::BN;
     const int t0 = split * p.per, t1 = min(tiles, t0 + p.per);
 
-    if constexpr (BIAS) bias.gather(p, head0);
+    if constexpr (BIAS) {
+        bias.even = even;
+        bias.gather(p, head0);
+    }
     const int64_t oo = (int64_t)b * p.ob + (int64_t)i * p.ldo + head * p.D;
     Frag<T, DP> q, go, o;
     q.load(p.Q, (int64_t)b * p.qb + (int64_t)i * p.ldq + head * p.D, rok, p.D, h);
@@ -874,7 +889,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
     tk.init(p.ldk, p.D, tid);
     tv.init(p.ldv, p.D, tid);
     Keys keys;
-    keys.start(p, b, kend, ring, t0 * C::BN, tid);
+    keys.start(p, b, even, kend, ring, t0 * C::BN, tid);
     auto issue = [&](int t) {
         const uint32_t img = (t - t0) % C::NS * 2 * C::IMG;
         const int k0 = t * C::BN, shift = C::BN < 64 ? k0 & 63 : 0;
@@ -949,6 +964,7 @@ __global__ void __launch_bounds__(256, (BwdQCfg<T, DP, WK, BIAS>::WAVES)) la_bac
 #pragma unroll
         for (int e = 0; e < 16; ++e) dq[dt][e] = 0.f;
 
+    if (even) q.clear();
     q.settle();
     go.settle();
     for (int t = t0; t < t1; ++t) {
@@ -1238,9 +1254,10 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     if constexpr (BIAS) bias.ask(p, 0, tid);
     const int kt = blockIdx.y, split = blockIdx.z, b = (int)(blockIdx.x / (unsigned)p.Hk), kvh = (int)blockIdx.x - b * p.Hk;
     const int kbase = kt * C::KEYS, wq = wave % WQ, kw = kbase + wave / WQ * 32, key = kw + (lane & 31);
-    int kend = visible_end(p, b);
+    bool even;
+    int kend = visible_end(p, b, even);
     if (p.causal) kend = min(kend, p.q_start + p.Sq);  // the last row's position: what lies behind it is visible to no row
-    const int seen = key < kend ? p.mask ? p.mask[(int64_t)b * p.Sk + key] : 1 : 0;
+    const int seen = key < kend ? p.mask && !even ? p.mask[(int64_t)b * p.Sk + key] : 1 : 0;
     const int64_t kvrow = (int64_t)b * p.kb + (int64_t)key * p.ldk + kvh * p.D, vrow = (int64_t)b * p.vb + (int64_t)key * p.ldv + kvh * p.D;
     const int64_t rows_all = (int64_t)p.B * p.H * p.Sq;
 
@@ -1248,7 +1265,10 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
     const int tiles = kbase < kend ? p.G * max(nq, 0) : 0;
     const int t0 = split * p.per, t1 = min(tiles, t0 + p.per);
     int gcur = t0 < t1 ? t0 / nq : 0;
-    if constexpr (BIAS) bias.gather(p, kvh * p.G + gcur);
+    if constexpr (BIAS) {
+        bias.even = even;
+        bias.gather(p, kvh * p.G + gcur);
+    }
     QT tq, tg;
     tq.init(p.ldq, p.D, tid);
     tg.init(p.lddo, p.D, tid);
@@ -1268,7 +1288,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         if (t0 + k < t1) issue(t0 + k);
 
     Frag<T, DP> kf, vf;
-    kf.load(p.K, kvrow, key < kend, p.D, h);
+    kf.load(p.K, kvrow, key < kend && !even, p.D, h);  // for the scores alone
     vf.load(p.V, vrow, key < kend, p.D, h);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
@@ -1325,7 +1345,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         else wait_copies<0>();
         barrier();
         if (BIAS && g != gcur) {  // another head of the group: its bias
-            bias_fill<T>(p, head, bv, tid);
+            bias_fill<T>(p, head, even, bv, tid);
             barrier();
             gcur = g;
         }

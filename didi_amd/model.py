@@ -343,11 +343,12 @@ class DiDiSampler:
         wide_heads = D > 64 or D % 8 != 0  # e.g. Blenderbot-3B's 80-wide heads (configs/train.yaml:3), t5-3b / t5-11b: d_kv = 128
         # past the sizes the attention kernels of a dialog are built for: fp32 attention of any length
         long = Cn > ops.ATTENTION_MAX_LEN or (wide_heads and not ops.attention_train_fits(Cn, Cn, D))
+        count32 = ops.additive_mask_counts(mask32) if long else None
 
         def attn(qkv_hi, qkv_lo, qkv_f32=None):
             v = lambda t, i: None if t is None else t.view(B, Cn, 3 * E)[:, :, i * E:(i + 1) * E]  # noqa: E731
             if long:
-                o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32)
+                o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32, key_count=count32)
                 return ops.split(o.view(B * Cn, E))
             if wide_heads:  # past the MFMA attention kernel's head dim: the fp32 LDS kernel of the training forward (cold path)
                 o = ops.attention_train(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, causal=False, key_mask=mask32)
@@ -376,7 +377,8 @@ class DiDiSampler:
             def attn_t5(qkv_hi, qkv_lo, qkv_f32=None):
                 v = lambda t, i: t.view(B, Cn, 3 * inner)[:, :, i * inner:(i + 1) * inner]  # noqa: E731
                 if long:
-                    o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32, scale=1.0, rel_bias=(e["rel"], buckets))
+                    o = ops.cross_attention(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, key_mask=mask32, key_count=count32, scale=1.0,
+                                            rel_bias=(e["rel"], buckets))
                     return ops.split(o.view(B * Cn, inner))
                 if wide_heads:
                     o = ops.attention_train(v(qkv_f32, 0), v(qkv_f32, 1), v(qkv_f32, 2), A, causal=False, key_mask=mask32, scale=1.0,

@@ -783,13 +783,19 @@ def _long_run(dev, what, fn, backward, fields):
     _lib.check(rc, what)
 
 
+def additive_mask_counts(mask32):
+    """int32 [B, Sk] mask -> ``key_count`` int32 [B] under which ``cross_attention`` does as additive masks of the lowest value do: a dialog whose mask
+    leaves nothing averages all values (as ``attention`` and ``attention_train`` do), the others go by the mask."""
+    return torch.where(mask32.any(1), mask32.shape[1], -1).to(torch.int32)
+
+
 def cross_attention(q, k, v, heads, kv_heads=None, causal=False, q_start=0, key_mask=None, key_count=None, scale=None, rel_bias=None, drop_p=0.0,
                     seed=0, offset=0, need_grad=False, out=None):
     """Attention of q [B, Sq, heads D] over k, v [B, Sk, kv_heads D] of any other length (self-attention: the same sequence) -> o like q.
 
     bf16, fp16 or fp32, all operands alike; views with strides between rows and dialogs are fine (16-byte aligned).  Head dims up to 128,
     multiples of 8 (fp32: 4).  ``kv_heads``: each key head serves heads / kv_heads query heads.  A key is visible where
-    ``key_mask`` int32 [B, Sk] is not 0, before ``key_count`` int32 [B], and (``causal``) up to position q_start + i; a row that sees none
+    ``key_mask`` int32 [B, Sk] is not 0, before ``key_count`` int32 [B] (negative: the dialog's rows average all its values), and (``causal``) up to position q_start + i; a row that sees none
     gives zeros, and what lies at keys that no row of a dialog sees is never used.  ``scale``: default 1/sqrt(D).  ``rel_bias`` = (table [num_buckets, heads],
     relative_buckets(...)): a learned bias by the distance from query q_start + i to the key, added to the scaled scores.  ``drop_p``,
     ``seed``, ``offset``: dropout of the probabilities, ``attention_train``'s mask.

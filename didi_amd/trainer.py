@@ -331,6 +331,7 @@ class DiDiTrainer:
         # ---- context: frozen encoder, trainable adapter (model.py:165-170, 183-188)
         c_hi, c_lo, enc = self.frozen._encode_raw(cids, cmask)
         mask32 = cmask.to(torch.int32).contiguous()
+        seen = dict(key_mask=mask32, key_count=ops.additive_mask_counts(mask32)) if long else dict(key_mask=mask32)
         if cfg.has_adapter:
             if pd != torch.bfloat16:
                 c_hi, c_lo = ops.split(enc, dtype=pd)
@@ -370,7 +371,7 @@ class DiDiTrainer:
             _, _, ckv = self._linear(L["ckv"], x_hi, x_lo, out_planes=False)
             kv3 = ckv.view(B, Cn, 2 * H)
             s["off_ca"] = site()
-            catt, s["stat_ca"] = attend(cq.view(B, S, H), kv3[:, :, :H], kv3[:, :, H:], key_mask=mask32, offset=s["off_ca"])
+            catt, s["stat_ca"] = attend(cq.view(B, S, H), kv3[:, :, :H], kv3[:, :, H:], offset=s["off_ca"], **seen)
             ca_hi, ca_lo = ops.split(catt, dtype=pd)
             s["cq"], s["ckv"], s["catt"], s["cattp"] = cq, ckv, catt, (ca_hi, ca_lo)
             s["off_co"] = site()
@@ -463,7 +464,7 @@ class DiDiTrainer:
             dckv = torch.empty_like(ckv)
             dcq = torch.empty((B, S, H), dtype=torch.float32, device=dev)
             attend_backward(s["cq"].view(B, S, H), ckv[:, :, :H], ckv[:, :, H:], s["catt"], s["stat_ca"], dcatt, (dcq, dckv[:, :, :H], dckv[:, :, H:]),
-                            key_mask=mask32, offset=s["off_ca"])
+                            offset=s["off_ca"], **seen)
             dh1, dW, dbias = self._linear_bwd(dcq.view(M, H), s["h1"], L["cq"], residual=ds2, A_planes=s["h1p"])
             put(ln["cq"], dW, dbias)
             dctx_l, dW, dbias = self._linear_bwd(dckv.view(B * Cn, 2 * H), ctx.view(B * Cn, H), L["ckv"], residual=dctx, need_dA=need_dctx, A_planes=(x_hi, x_lo))

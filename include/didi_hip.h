@@ -696,7 +696,7 @@ int didi_train_target_backward(const float* x0hat, const float* emb, const float
  *   visible(b, i, j) = j < key_count[b] and key_mask[b, j] != 0 and (not causal or j <= q_start + i)
  *   o_i = sum_j p_ij v_j,  p = dropout(softmax_j(scale q_i . k_j + table[buckets[clamp(j - q_start - i)]][head])) over the visible j
  * A row that sees no key gives o = 0, lse = -inf and no gradients (didi_attention's rows without a visible key average all values
- * instead), whatever its q and do hold; keys and values that no row of their dialog sees are never multiplied, whatever they hold, and get gradients
+ * instead: key_count < 0), whatever its q and do hold; keys and values that no row of their dialog sees are never multiplied, whatever they hold, and get gradients
  * of 0.  What causal hides from some rows only has to be finite.  NaN at visible places reaches o, lse and the gradients.
  * A table entry of -inf hides its distances, and so does one below -2.36e38 (scores are kept in base 2).  Statistics and sums are fp32: the backward's
  * probabilities are right to |lse| 2^-23, so what is to be hidden belongs in key_mask or at -inf, not at a large negative number.
@@ -716,7 +716,9 @@ typedef struct didi_long_attn_args {
     int causal, q_start;       /* query i stands at position q_start + i (causal limit and distances) */
     float scale;               /* 0 = 1/sqrt(D); otherwise 2^-126 .. 2^127 */
     const int32_t* key_mask;   /* [B, Sk] or NULL */
-    const int32_t* key_count;  /* [B] or NULL: keys from key_count[b] on are not visible */
+    const int32_t* key_count;  /* [B] or NULL: keys from key_count[b] on are not visible; negative: all Sk keys are, whatever key_mask says, and all scores
+                                  are 0 -- the mean of the values, to which additive masks of the lowest value come where they leave nothing; the gradients
+                                  are theirs, too: scores that are masked this way still pass theirs on to q, k and the table */
     const void *Q, *K, *V;
     int64_t q_batch, k_batch, v_batch;
     int ldq, ldk, ldv;

@@ -397,3 +397,51 @@ def test_seeds_are_taken_as_the_training_attention_takes_them(ops, seed, offset)
     a, b = ops.cross_attention(q, k, v, H, **kw), ops.attention_train(q, k, v, H, **kw)
     # probabilities to fp32's 32 + 8 roundings of scores of size 8 in both; another mask would differ by a probability, 0.05
     assert (a - b).abs().max() < 1e-4 and (a != ops.cross_attention(q, k, v, H)).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("H,Hk,Sq,Sk,D,bias,causal", [(4, 2, 1, 300, 64, False, False), (3, 3, 40, 130, 96, True, False), (4, 4, 130, 97, 64, False, False),
+                                                      (2, 1, 70, 5000, 32, False, False), (24, 24, 260, 130, 64, True, False), (2, 2, 50, 60, 128, False, True)])
+def test_a_negative_count_averages_the_values(ops, dtype, H, Hk, Sq, Sk, D, bias, causal):  # noqa: F811
+    """A dialog whose key count is negative has scores of 0 at all its keys, and the gradients of scores that a mask has been added to."""
+    B, G = 3, H // Hk
+    q, k, v, do = make(B, H, Hk, Sq, Sk, D, dtype, seed=16)
+    mask = (torch.rand(B, Sk, generator=torch.Generator().manual_seed(5)) < 0.7).int().cuda()
+    mask[1] = 0
+    count = torch.tensor([Sk, -1, (Sk + 1) // 2], dtype=torch.int32, device="cuda")
+    kw = dict(key_mask=mask, key_count=count, causal=causal, q_start=5 if causal else 0)
+    if bias:
+        table = torch.randn(32, H, generator=torch.Generator().manual_seed(3)).to(DT[dtype]).cuda()
+        kw["rel_bias"] = (table, ops.relative_buckets())
+    got, lse = run(ops, q, k, v, do, H, Hk, **kw)
+    # the other dialogs as ever
+    rest = {**kw, "key_mask": mask[::2].contiguous(), "key_count": count[::2].contiguous()}
+    val_rest, tol_rest = reference(*(x[::2].contiguous() for x in (q, k, v, do)), H, Hk, dtype, **rest)
+    for n in ("o", "dq", "dk", "dv"):
+        assert ((got[n][::2].double() - val_rest[n]).abs() <= tol_rest[n]).all(), n
+    # the dialog itself: scores of zero, by a scale of zero in the definition; dq and dk are then those of scale 1, times the scale
+    val, tol = reference(q[1:2] * 0, k[1:2], v[1:2], do[1:2], H, Hk, dtype, causal=causal, q_start=kw["q_start"])
+    assert ((got["o"][1:2].double() - val["o"]).abs() <= tol["o"]).all() and ((got["dv"][1:2].double() - val["dv"]).abs() <= tol["dv"]).all()
+    assert ((got["dq"][1:2].double() - val["dq"]).abs() <= tol["dq"]).all()
+    seen = torch.arange(Sk, device="cuda")[None] <= torch.arange(Sq, device="cuda")[:, None] + 5 if causal else torch.ones(Sq, Sk, dtype=torch.bool, device="cuda")
+    p = seen.double() / seen.sum(1, keepdim=True)
+    heads = lambda x, n: x[1].double().reshape(-1, n, D).transpose(0, 1)  # noqa: E731
+    dO, V, Q = heads(do, H), heads(v, Hk).repeat_interleave(G, 0), heads(q, H)
+    dp = dO @ V.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    by_head = lambda x: x.reshape(Hk, G, Sk, D).sum(1).transpose(0, 1).reshape(Sk, Hk * D)  # noqa: E731
+    dk = by_head(ds.transpose(-1, -2) @ Q) / math.sqrt(D)
+    # ds: rounded once, D = do . o to the remainder's or fp32's bits; then a sum over rows and heads, rounded once
+    u, lo = U[dtype], U[dtype] if dtype == "fp32" else U[dtype] ** 2
+    err = ds.abs() * (0 if dtype == "fp32" else u) + p * (dO.abs() @ V.abs().transpose(-1, -2) + (dO.abs() * (p @ V.abs())).sum(-1, keepdim=True)) * (
+        (0 if dtype == "fp32" else u) + lo + (D + Sk + 8) * 2.0 ** -24) + SUB[dtype] * 2.0 ** -6 * dO.norm(dim=-1).amax()
+    bound = by_head(err.transpose(-1, -2) @ Q.abs() + (G * Sq + 4) * 2.0 ** -24 * (ds.abs().transpose(-1, -2) @ Q.abs())) / math.sqrt(D) + u * dk.abs() + SUB[dtype]
+    assert ((got["dk"][1].double() - dk).abs() <= bound).all()
+    want = torch.log(seen.sum(1).double())
+    assert ((lse[1].double() - want).abs() <= 1e-5 * (1 + want)).all()
+    if bias:
+        hot = torch.nn.functional.one_hot(bucket_of(kw["rel_bias"][1], Sq, Sk, 0), 32).double().reshape(Sq * Sk, 32)
+        by = lambda x: (x.reshape(H, Sq * Sk) @ hot).t()  # noqa: E731
+        total = val_rest["dtable"] + by(ds)
+        slack = tol_rest["dtable"] + by(err + ds.abs() * (B * Sq + 4) * 2.0 ** -24) + u * total.abs() + SUB[dtype]
+        assert ((got["dtable"].double() - total).abs() <= slack).all()
