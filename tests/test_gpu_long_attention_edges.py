@@ -445,3 +445,24 @@ def test_a_negative_count_averages_the_values(ops, dtype, H, Hk, Sq, Sk, D, bias
         total = val_rest["dtable"] + by(ds)
         slack = tol_rest["dtable"] + by(err + ds.abs() * (B * Sq + 4) * 2.0 ** -24) + u * total.abs() + SUB[dtype]
         assert ((got["dtable"].double() - total).abs() <= slack).all()
+
+
+# Sizes at which a workgroup of the gradient takes 64 rows (16 a wave, two at a time, over and again), a row has more chunks than a wave reads at a
+# time (2048 columns of 16 bits, 1024 of fp32), or none: narrower than a chunk, or beyond the table's distances throughout
+@pytest.mark.parametrize("dtype,B,H,Sq,Sk,q_start,bidirectional", [
+    ("bf16", 1, 32, 4100, 2111, 7, True), ("fp16", 2, 32, 2100, 2053, 0, False), ("fp32", 1, 64, 2049, 1027, 5, True), ("bf16", 2, 33, 2000, 2603, 300, True),
+    ("fp32", 1, 32, 4200, 9, 0, True), ("fp16", 1, 32, 4200, 5, 0, True), ("bf16", 3, 16, 3001, 1, 0, False), ("fp16", 1, 64, 2050, 601, 4000, True),
+    ("fp32", 1, 1, 65, 300001, 0, True), ("bf16", 1, 2, 7, 200003, 100, True)])
+def test_long_gradient_of_the_bias(ops, dtype, B, H, Sq, Sk, q_start, bidirectional):  # noqa: F811
+    buckets = ops.relative_buckets(32, 128, bidirectional)
+    d = torch.randn(B, H, Sq, Sk, generator=torch.Generator(device="cuda").manual_seed(Sq), device="cuda").to(DT[dtype])
+    got = ops.relative_bias_backward(d, buckets, 32, q_start=q_start)
+    bucket = bucket_of(buckets, Sq, Sk, q_start)
+    other = [bucket != t for t in range(32)]
+    assert torch.equal(got, ops.relative_bias_backward(d, buckets, 32, q_start=q_start))
+    for h in range(H):
+        by = lambda x: torch.stack([x.masked_fill(other[t], 0.0).sum() for t in range(32)])  # noqa: E731
+        x = d[:, h].double()
+        want, size = by(x), by(x.abs())
+        # fp32 sums: a lane takes 64 rows of at most Sk / 64 elements, then partial sums of B Sq / 64 workgroups
+        assert ((got[:, h].double() - want).abs() <= size * (B * Sq + Sk + 16) * 2.0 ** -24 + U[dtype] * want.abs() + SUB[dtype]).all(), h
