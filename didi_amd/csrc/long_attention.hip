@@ -488,6 +488,7 @@ static int check_bias(const int32_t* buckets, int dtype, int heads, int num_buck
     DIDI_CHECK_ARG(dtype == DIDI_DT_BF16 || dtype == DIDI_DT_FP16 || dtype == DIDI_DT_FP32);
     const int64_t lim = (int64_t)1 << 30;
     if (max_distance > MAX_DIST || num_buckets > MAX_BUCKETS || heads > 65535 || Sk > lim || (int64_t)q_start + Sq > lim) return DIDI_ERR_UNSUPPORTED;
+    if ((int64_t)Sq * Sk > ((int64_t)1 << 40)) return DIDI_ERR_UNSUPPORTED;  // what the launch's grid holds, and more than any memory does
     return DIDI_OK;
 }
 

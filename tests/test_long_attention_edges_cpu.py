@@ -49,3 +49,9 @@ def test_rows_too_wide_for_a_tile_are_refused():
 @pytest.mark.parametrize("scale", [1e-40, 2.0 ** -149, 3e38, -1.0, float("nan")])
 def test_a_scale_that_fp32_cannot_hold_is_refused(scale):
     assert lib.didi_long_attention_forward(args(**{**APART, "scale": scale}), None) == -1
+
+
+def test_a_bias_larger_than_any_memory_is_refused():
+    for Sq, Sk in ((1 << 30, 1 << 30), (1 << 21, 1 << 20)):
+        assert lib.didi_relative_bias(MB, MB, 0, 4, 32, 128, Sq, Sk, 0, MB, None) == -2
+        assert lib.didi_relative_bias_backward(MB, MB, 0, 1, 4, 32, 128, Sq, Sk, 0, MB, MB, None) == -2
