@@ -262,11 +262,14 @@ def _load():
             "or `make -C didi_amd/csrc`.  didi_amd has no non-HIP fallback."
         )
     lib = C.CDLL(LIB_PATH)
-    for name, res, args in SYMBOLS:
-        fn = getattr(lib, name)  # AttributeError if the symbol is not exported
-        fn.restype, fn.argtypes = res, args
-    if lib.didi_version() != ABI_VERSION:
+    missing = [name for name, _, _ in SYMBOLS if not hasattr(lib, name)]
+    if "didi_version" not in missing and lib.didi_version() != ABI_VERSION:
         raise ImportError(f"libdidi_hip ABI version {lib.didi_version()} != {ABI_VERSION}")
+    if missing:  # functions are added without a new version: what was there keeps its meaning
+        raise ImportError(f"{LIB_PATH} was built from other sources, it lacks {', '.join(missing)}: build it again")
+    for name, res, args in SYMBOLS:
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
     # the library never reads the environment; the tools' DIDI_<OPTION>=<int> variables are applied here, through the ABI
     for name, key in OPTIONS.items():
         v = os.environ.get("DIDI_" + name)
