@@ -826,9 +826,9 @@ def cross_attention_backward(q, k, v, o, saved, dO, heads, kv_heads=None, causal
     lse, o_lo = saved
     if lse.shape != (shape[0], heads, shape[1]) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
         raise ValueError("saved must be what cross_attention returned for these operands")
-    if o_lo is not None and (o_lo.shape != shape or o_lo.stride() != o.stride()):
-        raise ValueError("o must be the tensor that cross_attention returned (or one laid out like it)")
     O, ob, ldo = _rows("o", o, shape, dt, dev)
+    if o_lo is not None and (dt == torch.float32 or _rows("saved", o_lo, shape, dt, dev)[1:] != (ob, ldo)):
+        raise ValueError("o must be the tensor that cross_attention returned (or one laid out like it)")
     G, gb, ldg = _rows("dO", dO, shape, dt, dev)
     if out is None:
         grads = (torch.empty(shape, dtype=dt, device=dev), torch.empty(kv_shape, dtype=dt, device=dev), torch.empty(kv_shape, dtype=dt, device=dev))

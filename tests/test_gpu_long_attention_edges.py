@@ -466,3 +466,23 @@ def test_long_gradient_of_the_bias(ops, dtype, B, H, Sq, Sk, q_start, bidirectio
         want, size = by(x), by(x.abs())
         # fp32 sums: a lane takes 64 rows of at most Sk / 64 elements, then partial sums of B Sq / 64 workgroups
         assert ((got[:, h].double() - want).abs() <= size * (B * Sq + Sk + 16) * 2.0 ** -24 + U[dtype] * want.abs() + SUB[dtype]).all(), h
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_what_was_saved_is_checked(ops, dtype):  # noqa: F811
+    q, k, v, do = make(2, 2, 2, 9, 12, 32, dtype)
+    o, (lse, lo) = ops.cross_attention(q, k, v, 2, need_grad=True)
+    bad = [(lse.cpu(), lo), (lse.double(), lo), (lse[:1], lo), (lse.transpose(1, 2), lo), (lse, torch.empty(2, 9, 64, dtype=DT[dtype])),
+           (lse, torch.empty(2, 9, 64, dtype=torch.float16, device="cuda")), (lse, torch.empty(2, 9, 128, dtype=DT[dtype], device="cuda")[:, :, :64])]
+    for saved in bad:
+        with pytest.raises(ValueError):
+            ops.cross_attention_backward(q, k, v, o, saved, do, 2)
+    # one dialog or one row: strides that do not count may differ
+    for x in ((q[:1], k[:1], v[:1], do[:1]), (q[:, :1], k, v, do[:, :1])):
+        x = [t.contiguous() for t in x]
+        o, saved = ops.cross_attention(*x[:3], 2, need_grad=True)
+        want = ops.cross_attention_backward(*x[:3], o, saved, x[3], 2)
+        B, S, W = o.shape
+        view = o.as_strided((B, S, W), (S * W if B > 1 else 8, W if S > 1 else 8, 1))
+        got = ops.cross_attention_backward(*x[:3], view, saved, x[3], 2)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
