@@ -486,3 +486,25 @@ def test_what_was_saved_is_checked(ops, dtype):  # noqa: F811
         view = o.as_strided((B, S, W), (S * W if B > 1 else 8, W if S > 1 else 8, 1))
         got = ops.cross_attention_backward(*x[:3], view, saved, x[3], 2)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_keys_past_four_gibibytes(ops):  # noqa: F811
+    """Rows, outputs and gradients whose offsets pass 32 bits: a few visible keys of a long cache, the last one among them, against the same keys alone."""
+    H, D, Sk = 16, 128, (1 << 20) + 4097  # 4 KiB a row
+    W = H * D
+    g = torch.Generator().manual_seed(17)
+    at = torch.tensor([0, 5, (1 << 19) - 1, 1 << 19, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, (1 << 20) + 64, Sk - 2, Sk - 1]).cuda()
+    k, v = (torch.full((1, Sk, W), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    few = [torch.randn(1, at.numel(), W, generator=g).bfloat16().cuda() for _ in range(2)]
+    k[:, at], v[:, at] = few
+    mask = torch.zeros(1, Sk, dtype=torch.int32, device="cuda")
+    mask[:, at] = 1
+    for Sq in (1, 65):
+        q, do = (torch.randn(1, Sq, W, generator=g).bfloat16().cuda() for _ in range(2))
+        val, tol = reference(q, few[0], few[1], do, H, H, "bf16")
+        o, saved = ops.cross_attention(q, k, v, H, key_mask=mask, need_grad=True)
+        dq, dk, dv = ops.cross_attention_backward(q, k, v, o, saved, do, H, key_mask=mask)
+        compare({"o": o, "dq": dq, "dk": dk[:, at], "dv": dv[:, at]}, val, tol)
+        for x in (dk, dv):
+            x[:, at] = 0
+            assert not x.any()
