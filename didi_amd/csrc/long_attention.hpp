@@ -1337,6 +1337,7 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         kf.clear();
         vf.clear();
     }
+    const bool some = __any(vis);
     kf.settle();
     vf.settle();
     for (int t = t0; t < t1; ++t) {
@@ -1352,21 +1353,23 @@ __global__ void __launch_bounds__(256, (BwdKCfg<T, DP, WQ>::WAVES)) la_backward_
         if (t + C::NS - 1 < t1) issue(t + C::NS - 1);
         const char *Qs = smem + (t - t0) % C::NS * (2 * C::IMG + C::STAT), *Gs = Qs + C::IMG;
         const float* rc = reinterpret_cast<const float*>(Gs + C::IMG + wave * 512);  // -lse log2(e) of the wave's rows, 64 on D
-        // rows that saw nothing are not multiplied either (their constants D and |do| are zeros): a wave clears what it is about to read itself, others
-        // that read the same rows do so too
-        if (uint64_t none = __ballot(rc[lane & (32 * C::NT - 1)] == -INFINITY) & (C::NT == 2 ? ~0ull : 0xffffffffull)) {
-            constexpr int CH = DP / T::EPC;
-            char* at = smem + (Qs - smem) + qrow * CH * 16 + lane * 16;
-            for (; none; none &= none - 1)
-                if (lane < CH) {
-                    const int to = __builtin_ctzll(none) * CH * 16;
-                    *reinterpret_cast<uint4*>(at + to) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(at + to + C::IMG) = make_uint4(0, 0, 0, 0);
-                }
-            asm volatile("" ::: "memory");
-        }
-        // a wave none of whose keys is seen by the tile's last row has nothing to add
-        if (!p.causal || kw <= p.q_start + min(i0 + qrow + 32 * C::NT, p.Sq) - 1) {
+        // a wave none of whose keys is seen, or seen by the tile's last row, has nothing to add
+        if (some && (!p.causal || kw <= p.q_start + min(i0 + qrow + 32 * C::NT, p.Sq) - 1)) {
+            // Rows that saw nothing are not multiplied either (their constants D and |do| are zeros): a wave clears what it is about to read itself, others
+            // that read the same rows do so too.  Without a causal limit and a bias every row of a dialog sees what its keys show, and looking for such
+            // rows would cost 2 % (2048 x 8192 of 128, one wave a SIMD: 30 of 1010 us).
+            uint64_t none = BIAS || p.causal ? __ballot(rc[lane & (32 * C::NT - 1)] == -INFINITY) & (C::NT == 2 ? ~0ull : 0xffffffffull) : 0;
+            if (none) {
+                constexpr int CH = DP / T::EPC;
+                char* at = smem + (Qs - smem) + qrow * CH * 16 + lane * 16;
+                for (; none; none &= none - 1)
+                    if (lane < CH) {
+                        const int to = __builtin_ctzll(none) * CH * 16;
+                        *reinterpret_cast<uint4*>(at + to) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(at + to + C::IMG) = make_uint4(0, 0, 0, 0);
+                    }
+                asm volatile("" ::: "memory");
+            }
             constexpr int UNROLL = DP > 64 ? 1 : C::NT;
 #pragma unroll UNROLL
             for (int nt = 0; nt < C::NT; ++nt) {
