@@ -520,7 +520,7 @@ constexpr int max_share(bool f32, int DP) { return f32 && DP > 64 ? 2 : 4; }
 // fewer rows, the waves' shares are joined through LDS at the end (small batches, one token per dialog).
 // What bounds it: one token per dialog, the reading of keys and values -- 32 dialogs x 12 heads to 4096 keys, fp16: 48 us, 4.3 TB/s; 4 x 32 heads
 // over 8 of 128, 33001 keys, bf16: 100 us and 5 to join the splits, 5.1 TB/s.  Many rows, the products with the softmax between them (a wave's
-// products wait for its exponentials; other waves fill in): 2 x 16 heads of 128, 2048 x 8192, bf16: 310 us, 740 TFLOP/s.  Between them latency: a
+// products wait for its exponentials; other waves fill in): 2 x 16 heads of 128, 2048 x 8192, bf16: 315 us, 728 TFLOP/s.  Between them latency: a
 // launch over 500 keys is a prologue of 4 us and eight tiles that come one behind the other (64 x 12 heads, 63 x 512, fp16: 19 us).
 template <class T, int DP, int WK>
 struct FwdCfg {
@@ -673,6 +673,8 @@ __global__ void __launch_bounds__(256, (FwdCfg<T, DP, WK>::WAVES)) la_forward(La
                     for (int e = 0; e < 4; ++e) s[4 * gq + e] *= k[e];
                 }
             }
+            // 16 bits: the probabilities are rounded once to the type that the matrix instructions take, which leaves outputs 1.3 to 1.4 times as far off as
+            // the rounding of the result alone; a product with their remainders besides would be half the forward's products again
             add<T, DP>(cv, s, o);
             if constexpr (!T::F32) {
                 // D = do . o of the backward wants an output without the rounding of the probabilities, so their remainders are multiplied too where
@@ -821,7 +823,7 @@ __device__ __forceinline__ float pow2_scale(float norm, int to) {
     return __builtin_bit_cast(float, (uint32_t)(127 + min(max(to - e, -100), 100)) << 23);
 }
 
-// Bound by the products: 2 x 16 heads of 128, 2048 x 8192, bf16: 375 us for its three, 916 TFLOP/s.  Short ones by latency: causal fp32 128 x 128,
+// Bound by the products: 2 x 16 heads of 128, 2048 x 8192, bf16: 373 us for its three, 921 TFLOP/s.  Short ones by latency: causal fp32 128 x 128,
 // 96 heads of 64: 21 us, a third of it before the first tile (rows, bias, the sums' zeros), the rest two tiles of 6000 cycles.
 template <class T, int DP, int WK, bool BIAS>
 struct BwdQCfg {
@@ -1221,7 +1223,7 @@ __global__ void __launch_bounds__(256) la_sum_parts(const float* part, int ns, i
 // ------------------------------------------------------------------ backward: dK, dV
 // A workgroup owns 128 keys of one key head, its waves 32 each (lane = key: K and V rows live in registers); it walks tiles of BQ rows of
 // Q and dO of every head of the group.  Bound by its four products and what they wait for: head dims past 64 (16 bits) hold dK, dV, K and V of a wave's
-// keys in 400 registers, so one wave a SIMD is all there is to hide an LDS read behind: 2 x 16 heads of 128, 2048 x 8192, bf16: 740 us, 619
+// keys in 400 registers, so one wave a SIMD is all there is to hide an LDS read behind: 2 x 16 heads of 128, 2048 x 8192, bf16: 736 us, 622
 // TFLOP/s.  One launch for dK and one for dV have two waves a SIMD, but five products: 800 us.
 template <class T, int DP, int WQ>
 struct BwdKCfg {
