@@ -526,6 +526,7 @@ extern "C" int didi_relative_bias_backward(const void* dbias, const int32_t* buc
     if (const int rc = check_bias(buckets, dtype, heads, num_buckets, max_distance, Sq, Sk, q_start)) return rc;
     DIDI_CHECK_ARG(B >= 0 && dtable);
     const bool any = B > 0 && Sq > 0 && Sk > 0;
+    const int elem = dtype == DIDI_DT_FP32 ? 4 : 2;  // the loads need no more
     if ((int64_t)B * heads > 65535) return DIDI_ERR_UNSUPPORTED;
     hipStream_t st = as_stream(stream);
     LaParams p{};
@@ -533,7 +534,7 @@ extern "C" int didi_relative_bias_backward(const void* dbias, const int32_t* buc
     p.tpart = static_cast<float*>(workspace);
     int parts = 0;
     if (any && grad_small(B, Sq, Sk)) {
-        DIDI_CHECK_ARG(dbias && (reinterpret_cast<uintptr_t>(dbias) & 15) == 0);
+        DIDI_CHECK_ARG(dbias && reinterpret_cast<uintptr_t>(dbias) % elem == 0);
 #define DIDI_SMALL(T) la_bias_grad_small<T><<<heads, 512, (size_t)(Sq + Sk - 1) * 8, st>>>(dbias, buckets, heads, num_buckets, max_distance, Sq, Sk, q_start, dtable)
         if (dtype == DIDI_DT_FP32) DIDI_SMALL(EF32);
         else if (dtype == DIDI_DT_FP16) DIDI_SMALL(E16<true>);
@@ -543,7 +544,7 @@ extern "C" int didi_relative_bias_backward(const void* dbias, const int32_t* buc
         return DIDI_OK;
     }
     if (any) {
-        DIDI_CHECK_ARG(dbias && workspace && (reinterpret_cast<uintptr_t>(dbias) & 15) == 0);
+        DIDI_CHECK_ARG(dbias && workspace && reinterpret_cast<uintptr_t>(dbias) % elem == 0);
         const int rows = grad_rows((int64_t)B * heads, Sq);
         parts = cdiv(Sq, rows);
         const dim3 grid(parts, B * heads);

@@ -508,3 +508,13 @@ def test_keys_past_four_gibibytes(ops):  # noqa: F811
         for x in (dk, dv):
             x[:, at] = 0
             assert not x.any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("H,Sq,Sk", [(3, 7, 9), (1, 77, 301), (5, 133, 1023)])
+def test_gradient_of_the_bias_from_one_dialog_of_many(ops, dtype, H, Sq, Sk):  # noqa: F811
+    """A contiguous dialog whose first element lies anywhere in memory."""
+    buckets = ops.relative_buckets(32, 128)
+    d = torch.randn(3, H, Sq, Sk, generator=torch.Generator().manual_seed(Sk)).to(DT[dtype]).cuda()
+    for b in range(3):
+        assert torch.equal(ops.relative_bias_backward(d[b], buckets, 32), ops.relative_bias_backward(d[b].clone(), buckets, 32))
